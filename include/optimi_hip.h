@@ -336,6 +336,67 @@ int64_t optimi_hip_resident_launch_count(void);
  * Returns the limit that was in force before.  Results never depend on it. */
 int64_t optimi_hip_launch_limit(int64_t workgroups);
 
+/* ---------------------------------------------------------------------------------
+ * Activations in 8 bits.  No counterpart in the reference: these operators serve the training
+ * step around the optimizer - the activations that the backward pass keeps and the products
+ * around them.
+ *
+ * An int8 activation is a row-major [rows, cols] matrix of values in [-127, 127] with one fp32
+ * scale per row (per token, or per output channel of a weight): element (r, c) stands for
+ * values[r][c] * scales[r].  The library's own scales are powers of two - the smallest s with
+ * absmax <= 127 s, 1 for rows of zeros, never below 2^-126 - so a value's meaning is exact in every
+ * type; values stay within +-63 under scales whose 64th multiple the type cannot hold.  A row
+ * that holds an infinity or a NaN gets the scale NaN and zeros.  The products take any scales.
+ *
+ * All matrices are contiguous, rows < 2^31, cols <= 2^28 (OPTIMI_ERR_SIZE beyond).  Buffers need
+ * only be aligned to their element size.  Workspaces are the caller's: as many bytes of device memory
+ * as the _workspace function of the same name and sizes says (it returns a negative status for
+ * sizes that the call would refuse), aligned to 16 bytes, not shared by calls that may
+ * run at the same time, free again when the call's work on `stream` is done; NULL where that is 0.
+ * Nothing is allocated, cached or waited for, and every call may be captured into a HIP graph.
+ * ------------------------------------------------------------------------------- */
+
+/* values, scales of x. */
+int optimi_hip_int8_quantize(const void* x, int64_t rows, int64_t cols, int dtype, int8_t* values, float* scales,
+                             optimi_stream_t stream);
+
+/* out[r][c] = values[r][c] * scales[r], rounded to `dtype`. */
+int optimi_hip_int8_dequantize(const int8_t* values, const float* scales, int64_t rows, int64_t cols, int dtype, void* out,
+                               optimi_stream_t stream);
+
+/* out[m][n] = a_scales[m] * b_scales[n] * sum_k a[m][k] * b[n][k] (+ bias[n]), a [m, k], b [n, k], out and bias of
+ * `dtype`, bias may be NULL.  The sum is formed in whole numbers of 32 bits and is exact; k <= 131071, which keeps it
+ * there for all int8 values (OPTIMI_ERR_SIZE beyond). */
+int64_t optimi_hip_int8_matmul_workspace(int64_t m, int64_t n, int64_t k);
+int optimi_hip_int8_matmul(const int8_t* a, const float* a_scales, const int8_t* b, const float* b_scales, const void* bias,
+                           int64_t m, int64_t n, int64_t k, int dtype, void* out, void* workspace, optimi_stream_t stream);
+
+/* The gradient of a linear layer's weight from the int8 checkpoint of its input:
+ * weight_grad[n][k] = sum_r grad[r][n] * scales[r] * values[r][k], and bias_grad[n] = sum_r grad[r][n] where bias_grad
+ * is not NULL.  grad [rows, outs], values [rows, cols], weight_grad [outs, cols]; all but values and scales are of
+ * `dtype`.  Products of bf16 and fp16 gradients are formed with values[r][k] * scales[r] rounded to that type (exact
+ * for this library's scales), those of fp32 gradients without rounding; sums are fp32.  rows = 0 writes zeros. */
+int64_t optimi_hip_int8_weight_grad_workspace(int64_t rows, int64_t outs, int64_t cols, int dtype, int with_bias);
+int optimi_hip_int8_weight_grad(const void* grad, const int8_t* values, const float* scales, int64_t rows, int64_t outs,
+                                int64_t cols, int dtype, void* weight_grad, void* bias_grad, void* workspace,
+                                optimi_stream_t stream);
+
+/* h = x + residual (rounded to `dtype`; x itself, and h not written, where residual is NULL),
+ * rstd[r] = 1 / sqrt(mean(h[r]^2) + eps), and the int8 form of y[r][c] = h[r][c] * rstd[r] * weight[c], which is
+ * formed in fp32 and not rounded before.  weight is of `weight_dtype`: `dtype` or OPTIMI_F32.  cols >= 1. */
+int optimi_hip_add_rms_norm_int8(const void* x, const void* residual, const void* weight, int64_t rows, int64_t cols,
+                                 int dtype, int weight_dtype, double eps, void* h, int8_t* values, float* scales, float* rstd,
+                                 optimi_stream_t stream);
+
+/* Backward pass of the norm, y's gradient `grad` taken as if y had not been rounded to int8:
+ * dx = grad_h + rstd * (grad * weight - xhat * mean(grad * weight * xhat)), xhat = h * rstd - the gradient of x and
+ * of residual alike - and dweight = sum over rows of grad * xhat, in weight's type.  grad_h, what arrives on h
+ * itself, may be NULL. */
+int64_t optimi_hip_add_rms_norm_int8_backward_workspace(int64_t rows, int64_t cols);
+int optimi_hip_add_rms_norm_int8_backward(const void* grad, const void* grad_h, const void* h, const float* rstd,
+                                          const void* weight, int64_t rows, int64_t cols, int dtype, int weight_dtype,
+                                          void* dx, void* dweight, void* workspace, optimi_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

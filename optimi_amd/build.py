@@ -1,6 +1,6 @@
 """In-tree build of the two native pieces.
 
-* ``liboptimi_hip.so`` – the gfx950 kernels and the C ABI (hipcc, no torch).
+* ``liboptimi_hip.so`` – the gfx950 kernels and the C ABI (hipcc, no torch), one object per ``.hip`` source.
 * ``_C.*.so``          – the PyTorch-ROCm binding over that ABI (g++, host code only).
 
 Both land next to this file so they travel with the source tree.  Run
@@ -34,9 +34,11 @@ ROCM_HOME = os.environ.get("ROCM_HOME", "/opt/rocm")
 # and puts LDS reads into the element loops (fp32 AdamW over a cache-resident list: 74.5 us
 # with the pass, 67.5 us without; the 16-bit kernels are unchanged within noise).
 HIPCC_FLAGS = [
-    "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared", "-ffp-contract=off",
+    "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-mllvm", "-disable-vector-combine",
 ]
+KERNEL_SOURCES = ["optimi_hip.hip", "int8_rows.hip", "int8_gemm.hip"]
+BINDING_SOURCES = ["torch_binding.cpp", "int8_binding.cpp"]
 
 
 def _run(cmd: list[str]):
@@ -46,12 +48,47 @@ def _run(cmd: list[str]):
     return proc
 
 
-def build_lib(verbose: bool = False) -> str:
+def _lib_commands():
+    """Compile commands, link command and objects of the kernel library."""
     hipcc = shutil.which("hipcc") or os.path.join(ROCM_HOME, "bin", "hipcc")
-    cmd = [hipcc, *HIPCC_FLAGS, f"-I{INCLUDE}", "-o", LIB_PATH, os.path.join(CSRC, "optimi_hip.hip")]
+    objs = [os.path.join(CSRC, src[:-len(".hip")] + ".hip.o") for src in KERNEL_SOURCES]
+    compile_cmds = [[hipcc, *HIPCC_FLAGS, f"-I{INCLUDE}", "-c", os.path.join(CSRC, src), "-o", obj]
+                    for src, obj in zip(KERNEL_SOURCES, objs)]
+    return compile_cmds, [hipcc, "--offload-arch=gfx950", "-shared", *objs, "-o", LIB_PATH], objs
+
+
+def _remove(paths):
+    for path in paths:
+        if os.path.exists(path):
+            os.remove(path)
+
+
+def _compile_all(cmds, verbose: bool):
+    from concurrent.futures import ThreadPoolExecutor
+
+    with ThreadPoolExecutor(max_workers=max(1, len(cmds))) as pool:
+        jobs = []
+        for cmd in cmds:
+            if verbose:
+                print(" ".join(cmd))
+            jobs.append(pool.submit(_run, cmd))
+        for job in jobs:
+            job.result()
+
+
+def _link(cmd, verbose: bool):
     if verbose:
         print(" ".join(cmd))
     _run(cmd)
+
+
+def build_lib(verbose: bool = False) -> str:
+    compile_cmds, link_cmd, objs = _lib_commands()
+    try:
+        _compile_all(compile_cmds, verbose)
+        _link(link_cmd, verbose)
+    finally:
+        _remove(objs)
     return LIB_PATH
 
 
@@ -64,55 +101,43 @@ def _binding_commands():
     torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
     gxx = shutil.which("g++") or "g++"
-    obj = os.path.join(CSRC, "torch_binding.o")
-    compile_cmd = [
+    objs = [os.path.join(CSRC, src[:-len(".cpp")] + ".o") for src in BINDING_SOURCES]
+    compile_cmds = [[
         gxx, "-O2", "-std=c++17", "-fPIC", "-c", "-Wno-deprecated-declarations",
         "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
-        f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *inc, os.path.join(CSRC, "torch_binding.cpp"), "-o", obj,
-    ]
+        f"-D_GLIBCXX_USE_CXX11_ABI={abi}", *inc, os.path.join(CSRC, src), "-o", obj,
+    ] for src, obj in zip(BINDING_SOURCES, objs)]
     link_cmd = [
-        gxx, "-shared", obj, "-o", BINDING_PATH,
+        gxx, "-shared", *objs, "-o", BINDING_PATH,
         f"-L{HERE}", "-loptimi_hip", f"-L{torch_lib}", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip",
         "-ltorch_python", f"-L{ROCM_HOME}/lib", "-lamdhip64", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}",
         f"-Wl,-rpath,{ROCM_HOME}/lib",
     ]
-    return compile_cmd, link_cmd, obj
+    return compile_cmds, link_cmd, objs
 
 
 def build_binding(verbose: bool = False) -> str:
     """Compiles and links the binding; the kernel library must exist already (it is linked against)."""
-    compile_cmd, link_cmd, obj = _binding_commands()
+    compile_cmds, link_cmd, objs = _binding_commands()
     try:
-        for cmd in (compile_cmd, link_cmd):
-            if verbose:
-                print(" ".join(cmd))
-            _run(cmd)
+        _compile_all(compile_cmds, verbose)
+        _link(link_cmd, verbose)
     finally:
-        if os.path.exists(obj):
-            os.remove(obj)
+        _remove(objs)
     return BINDING_PATH
 
 
 def build_all(verbose: bool = False):
-    """Both pieces; the binding's translation unit compiles while hipcc works on the kernels,
-    and is linked once the library it links against is there."""
-    from concurrent.futures import ThreadPoolExecutor
-
-    compile_cmd, link_cmd, obj = _binding_commands()
+    """Both pieces: all translation units compile side by side, then the library is linked, then the
+    binding that is linked against it."""
+    lib_cmds, lib_link, lib_objs = _lib_commands()
+    binding_cmds, binding_link, binding_objs = _binding_commands()
     try:
-        with ThreadPoolExecutor(max_workers=2) as pool:
-            lib = pool.submit(build_lib, verbose)
-            if verbose:
-                print(" ".join(compile_cmd))
-            binding = pool.submit(_run, compile_cmd)
-            lib.result()
-            binding.result()
-        if verbose:
-            print(" ".join(link_cmd))
-        _run(link_cmd)
+        _compile_all(lib_cmds + binding_cmds, verbose)
+        _link(lib_link, verbose)
+        _link(binding_link, verbose)
     finally:
-        if os.path.exists(obj):
-            os.remove(obj)
+        _remove(lib_objs + binding_objs)
 
 
 if __name__ == "__main__":

@@ -56,6 +56,15 @@ PROTOTYPES = {
     "optimi_hip_upload_count": (_i64, []),
     "optimi_hip_resident_launch_count": (_i64, []),
     "optimi_hip_launch_limit": (_i64, [_i64]),
+    "optimi_hip_int8_quantize": (_i, [_p, _i64, _i64, _i, _p, _p, _p]),
+    "optimi_hip_int8_dequantize": (_i, [_p, _p, _i64, _i64, _i, _p, _p]),
+    "optimi_hip_int8_matmul_workspace": (_i64, [_i64, _i64, _i64]),
+    "optimi_hip_int8_matmul": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i, _p, _p, _p]),
+    "optimi_hip_int8_weight_grad_workspace": (_i64, [_i64, _i64, _i64, _i, _i]),
+    "optimi_hip_int8_weight_grad": (_i, [_p, _p, _p, _i64, _i64, _i64, _i, _p, _p, _p, _p]),
+    "optimi_hip_add_rms_norm_int8": (_i, [_p, _p, _p, _i64, _i64, _i, _i, _d, _p, _p, _p, _p, _p]),
+    "optimi_hip_add_rms_norm_int8_backward_workspace": (_i64, [_i64, _i64]),
+    "optimi_hip_add_rms_norm_int8_backward": (_i, [_p, _p, _p, _p, _p, _i64, _i64, _i, _i, _p, _p, _p, _p]),
 }
 
 _lib = None

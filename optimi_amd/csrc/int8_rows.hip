@@ -1,0 +1,644 @@
+// Row kernels of the int8 activations for MI355X (gfx950): quantize, dequantize, the residual add with RMS norm
+// and int8 output, and its backward pass.
+//
+// All of them stream: every input is read once, every output written once, and HBM bandwidth is the bound.  What
+// stands in the way is that a row's scale (and the norm's 1/rms) is known only after the whole row was seen.  A row
+// therefore stays in the registers of the team of lanes that works on it - one wavefront for short rows, a workgroup
+// of four for longer ones - between the reduction and the use of its result; only rows beyond 16384 elements are
+// read again (the second read is served by L2).  Sums, the norm's statistics and the quantized values are formed in
+// fp32 whatever the type of the tensors.
+
+#include "int8_common.h"
+
+namespace {
+
+using namespace optimi_int8;
+
+constexpr int kBlock = 256;           // lanes of a workgroup; 256 / TEAM rows are in work at once
+constexpr int kWaveRowCols = 1024;    // rows up to here belong to one wavefront: no LDS, no barrier
+constexpr int kLongCols = 8 * kBlock * 8;  // rows beyond 16384 elements do not stay in registers
+
+// Grids stay far below the 2^32 threads that a launch may have; a workgroup takes further rows in a loop.
+constexpr int64_t kMaxBlocks = 1 << 20;
+inline unsigned blocks_for(int64_t rows, int per_block) {
+  const int64_t n = (rows + per_block - 1) / per_block;
+  return (unsigned)(n < kMaxBlocks ? n : kMaxBlocks);
+}
+
+// A row of up to 8 * TEAM * VPT elements, vector v of lane l at element (v * TEAM + l) * 8.
+template <int TEAM>
+struct Place {
+  int lane;     // in the team
+  int64_t row;  // the team's first row
+  int64_t step; // rows that the whole grid takes at once
+  __device__ __forceinline__ Place() {
+    lane = threadIdx.x % TEAM;
+    row = (int64_t)blockIdx.x * (kBlock / TEAM) + threadIdx.x / TEAM;
+    step = (int64_t)gridDim.x * (kBlock / TEAM);
+  }
+};
+
+template <int DT, int TEAM, int VPT>
+__global__ void __launch_bounds__(kBlock) quantize_kernel(const typename Elem<DT>::type* __restrict__ x, int64_t rows, int64_t cols,
+                                                          int8_t* __restrict__ values, float* __restrict__ scales) {
+  using E = Elem<DT>;
+  __shared__ uint32_t slots[2][kBlock / 64];
+  const Place<TEAM> at;
+  // a team of four waves has the workgroup to itself, so all of its waves make the same number of rounds
+  int turn = 0;
+  for (int64_t row = at.row; row < rows; row += at.step, turn ^= 1) {
+    const typename E::type* in = x + row * cols;
+    typename E::Raw raw[VPT];
+    uint32_t most = 0;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int64_t c = (int64_t)(v * TEAM + at.lane) * 8;
+      raw[v] = c < cols ? load_some<DT>(in + c, cols - c) : E::zero();
+    }
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      float f[8];
+      E::unpack(raw[v], f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = MaxOp::join(most, abs_bits(f[i]));
+    }
+    most = team_reduce<MaxOp, TEAM>(most, slots[turn]);
+    const RowScale s = row_scale<DT>(most);
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int64_t c = (int64_t)(v * TEAM + at.lane) * 8;
+      float f[8];
+      E::unpack(raw[v], f);
+      if (c < cols) store_values(values + row * cols + c, quantize8(f, s), cols - c);
+    }
+    if (at.lane == 0) scales[row] = s.scale;
+  }
+}
+
+// Rows that do not fit the registers: one workgroup each, read twice.
+template <int DT>
+__global__ void __launch_bounds__(kBlock) quantize_long_kernel(const typename Elem<DT>::type* __restrict__ x, int64_t rows, int64_t cols,
+                                                               int8_t* __restrict__ values, float* __restrict__ scales) {
+  using E = Elem<DT>;
+  __shared__ uint32_t slots[2][kBlock / 64];
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
+    const typename E::type* in = x + row * cols;
+    uint32_t most = 0;
+    for (int64_t c = (int64_t)threadIdx.x * 8; c < cols; c += kBlock * 8) {
+      float f[8];
+      E::unpack(load_some<DT>(in + c, cols - c), f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = MaxOp::join(most, abs_bits(f[i]));
+    }
+    most = team_reduce<MaxOp, kBlock>(most, slots[turn]);
+    const RowScale s = row_scale<DT>(most);
+    for (int64_t c = (int64_t)threadIdx.x * 8; c < cols; c += kBlock * 8) {
+      float f[8];
+      E::unpack(load_some<DT>(in + c, cols - c), f);
+      store_values(values + row * cols + c, quantize8(f, s), cols - c);
+    }
+    if (threadIdx.x == 0) scales[row] = s.scale;
+  }
+}
+
+// q * s, eight values a lane; `team` lanes (a power of two) share a row.
+template <int DT>
+__global__ void __launch_bounds__(kBlock) dequantize_kernel(const int8_t* __restrict__ values, const float* __restrict__ scales, int64_t rows,
+                                                            int64_t cols, int team, typename Elem<DT>::type* __restrict__ out) {
+  const int lane = threadIdx.x % team;
+  for (int64_t row = (int64_t)blockIdx.x * (kBlock / team) + threadIdx.x / team; row < rows; row += (int64_t)gridDim.x * (kBlock / team)) {
+    const float s = scales[row];
+    for (int64_t c = (int64_t)lane * 8; c < cols; c += team * 8) {
+      const int8_t* p = values + row * cols + c;
+      float f[8];
+      if (cols - c >= 8) {
+        const u32x2 q = *(const u32x2_align1*)p;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = (float)(int8_t)(q[i / 4] >> (8 * (i % 4))) * s;
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = i < cols - c ? (float)p[i] * s : 0.0f;
+      }
+      store_some<DT>(out + row * cols + c, f, cols - c);
+    }
+  }
+}
+
+// The norm's weight in its own type: that of the activations or fp32.
+template <int DT, bool W32>
+struct Weight {
+  static constexpr int kType = W32 ? (int)OPTIMI_F32 : DT;
+  using E = Elem<kType>;
+  static __device__ __forceinline__ void load(const void* w, int64_t c, int64_t cols, float (&f)[8]) {
+    E::unpack(load_some<kType>((const typename E::type*)w + c, cols - c), f);
+  }
+};
+
+// h = x + residual, rounded to the type it is kept in; the norm is that of the kept values, which is what the
+// backward pass will see.
+template <int DT>
+__device__ __forceinline__ typename Elem<DT>::Raw add_rows(const typename Elem<DT>::Raw& x, const typename Elem<DT>::Raw& r) {
+  float a[8], b[8];
+  Elem<DT>::unpack(x, a);
+  Elem<DT>::unpack(r, b);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a[i] += b[i];
+  return Elem<DT>::pack(a);
+}
+
+struct NormArgs {
+  const void *x, *residual, *weight;
+  int64_t rows, cols;
+  float eps;
+  void* h;
+  int8_t* values;
+  float *scales, *rstd;
+};
+
+__device__ __forceinline__ float inverse_rms(float sum_of_squares, int64_t cols, float eps) {
+  return 1.0f / sqrtf(sum_of_squares / (float)cols + eps);
+}
+
+template <int DT, bool W32, int TEAM, int VPT>
+__global__ void __launch_bounds__(kBlock) norm_kernel(NormArgs a) {
+  using E = Elem<DT>;
+  using T = typename E::type;
+  __shared__ uint32_t slots[2][2][kBlock / 64];
+  const Place<TEAM> at;
+  int turn = 0;
+  for (int64_t row = at.row; row < a.rows; row += at.step, turn ^= 1) {
+    typename E::Raw raw[VPT];
+    float sum = 0.0f;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int64_t c = (int64_t)(v * TEAM + at.lane) * 8;
+      raw[v] = c < a.cols ? load_some<DT>((const T*)a.x + row * a.cols + c, a.cols - c) : E::zero();
+    }
+    if (a.residual) {
+#pragma unroll
+      for (int v = 0; v < VPT; ++v) {
+        const int64_t c = (int64_t)(v * TEAM + at.lane) * 8;
+        if (c < a.cols) {
+          raw[v] = add_rows<DT>(raw[v], load_some<DT>((const T*)a.residual + row * a.cols + c, a.cols - c));
+          float f[8];
+          E::unpack(raw[v], f);
+          store_some<DT>((T*)a.h + row * a.cols + c, f, a.cols - c);
+        }
+      }
+    }
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      float f[8];
+      E::unpack(raw[v], f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = fmaf(f[i], f[i], sum);
+    }
+    sum = __uint_as_float(team_reduce<SumOp, TEAM>(__float_as_uint(sum), slots[turn][0]));
+    const float r = inverse_rms(sum, a.cols, a.eps);
+    uint32_t most = 0;
+    float y[VPT][8];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int64_t c = (int64_t)(v * TEAM + at.lane) * 8;
+      float f[8], w[8];
+      E::unpack(raw[v], f);
+      if (c < a.cols) {
+        Weight<DT, W32>::load(a.weight, c, a.cols, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          y[v][i] = f[i] * r * w[i];
+          most = MaxOp::join(most, abs_bits(y[v][i]));
+        }
+      }
+    }
+    most = team_reduce<MaxOp, TEAM>(most, slots[turn][1]);
+    const RowScale s = row_scale<OPTIMI_F32>(most);
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int64_t c = (int64_t)(v * TEAM + at.lane) * 8;
+      if (c < a.cols) store_values(a.values + row * a.cols + c, quantize8(y[v], s), a.cols - c);
+    }
+    if (at.lane == 0) {
+      a.scales[row] = s.scale;
+      a.rstd[row] = r;
+    }
+  }
+}
+
+template <int DT, bool W32>
+__global__ void __launch_bounds__(kBlock) norm_long_kernel(NormArgs a) {
+  using E = Elem<DT>;
+  using T = typename E::type;
+  __shared__ uint32_t slots[2][2][kBlock / 64];
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    const T* x = (const T*)a.x + row * a.cols;
+    const T* res = a.residual ? (const T*)a.residual + row * a.cols : nullptr;
+    auto kept = [&](int64_t c, float (&f)[8]) {  // h, formed again from its two terms wherever it is needed
+      typename E::Raw raw = load_some<DT>(x + c, a.cols - c);
+      if (res) raw = add_rows<DT>(raw, load_some<DT>(res + c, a.cols - c));
+      E::unpack(raw, f);
+    };
+    float sum = 0.0f;
+    for (int64_t c = (int64_t)threadIdx.x * 8; c < a.cols; c += kBlock * 8) {
+      float f[8];
+      kept(c, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = fmaf(f[i], f[i], sum);
+    }
+    sum = __uint_as_float(team_reduce<SumOp, kBlock>(__float_as_uint(sum), slots[turn][0]));
+    const float r = inverse_rms(sum, a.cols, a.eps);
+    uint32_t most = 0;
+    for (int64_t c = (int64_t)threadIdx.x * 8; c < a.cols; c += kBlock * 8) {
+      float f[8], w[8];
+      kept(c, f);
+      Weight<DT, W32>::load(a.weight, c, a.cols, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = MaxOp::join(most, abs_bits(f[i] * r * w[i]));
+    }
+    most = team_reduce<MaxOp, kBlock>(most, slots[turn][1]);
+    const RowScale s = row_scale<OPTIMI_F32>(most);
+    for (int64_t c = (int64_t)threadIdx.x * 8; c < a.cols; c += kBlock * 8) {
+      float f[8], w[8], y[8];
+      kept(c, f);
+      Weight<DT, W32>::load(a.weight, c, a.cols, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] = f[i] * r * w[i];
+      store_values(a.values + row * a.cols + c, quantize8(y, s), a.cols - c);
+      if (res) store_some<DT>((T*)a.h + row * a.cols + c, f, a.cols - c);
+    }
+    if (threadIdx.x == 0) {
+      a.scales[row] = s.scale;
+      a.rstd[row] = r;
+    }
+  }
+}
+
+// Backward pass of y = h r w with r = (mean h^2 + eps)^(-1/2), g = dL/dy:
+//   dL/dh_i = r (g_i w_i - xhat_i mean(g w xhat)),  xhat = h r,  plus what arrives on the residual path;
+//   dL/dw_i = sum over rows of g_i xhat_i.
+// The second sum runs over rows: each team adds up its own rows in registers and leaves one partial row in the
+// workspace, and a second launch adds the partial rows in a fixed order - no atomics, the same bits on every run.
+struct NormBackwardArgs {
+  const void *grad, *grad_h, *h, *weight;
+  const float* rstd;
+  int64_t rows, cols;
+  void* dx;
+  float* partial;  // [teams][cols]
+};
+
+template <int DT, bool W32, int TEAM, int VPT>
+__global__ void __launch_bounds__(kBlock) norm_backward_kernel(NormBackwardArgs a) {
+  using E = Elem<DT>;
+  using T = typename E::type;
+  __shared__ uint32_t slots[2][kBlock / 64];
+  const Place<TEAM> at;
+  float w[VPT][8], dw[VPT][8];
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    const int64_t c = (int64_t)(v * TEAM + at.lane) * 8;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[v][i] = dw[v][i] = 0.0f;
+    if (c < a.cols) Weight<DT, W32>::load(a.weight, c, a.cols, w[v]);
+  }
+  int turn = 0;
+  for (int64_t row = at.row; row < a.rows; row += at.step, turn ^= 1) {
+    typename E::Raw g[VPT], h[VPT], more[VPT];
+    const float r = a.rstd[row];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int64_t c = (int64_t)(v * TEAM + at.lane) * 8;
+      g[v] = h[v] = more[v] = E::zero();
+      if (c < a.cols) {
+        g[v] = load_some<DT>((const T*)a.grad + row * a.cols + c, a.cols - c);
+        h[v] = load_some<DT>((const T*)a.h + row * a.cols + c, a.cols - c);
+        if (a.grad_h) more[v] = load_some<DT>((const T*)a.grad_h + row * a.cols + c, a.cols - c);
+      }
+    }
+    float dot = 0.0f;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      float fg[8], fh[8];
+      E::unpack(g[v], fg);
+      E::unpack(h[v], fh);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float xhat = fh[i] * r;
+        dw[v][i] = fmaf(fg[i], xhat, dw[v][i]);
+        dot = fmaf(fg[i] * w[v][i], xhat, dot);
+      }
+    }
+    dot = __uint_as_float(team_reduce<SumOp, TEAM>(__float_as_uint(dot), slots[turn]));
+    const float mean = dot / (float)a.cols;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+      const int64_t c = (int64_t)(v * TEAM + at.lane) * 8;
+      float fg[8], fh[8], fm[8], d[8];
+      E::unpack(g[v], fg);
+      E::unpack(h[v], fh);
+      E::unpack(more[v], fm);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) d[i] = fmaf(r, fg[i] * w[v][i] - fh[i] * r * mean, fm[i]);
+      if (c < a.cols) store_some<DT>((T*)a.dx + row * a.cols + c, d, a.cols - c);
+    }
+  }
+  const int64_t team = (int64_t)blockIdx.x * (kBlock / TEAM) + threadIdx.x / TEAM;
+#pragma unroll
+  for (int v = 0; v < VPT; ++v) {
+    const int64_t c = (int64_t)(v * TEAM + at.lane) * 8;
+    if (c < a.cols) store_some<OPTIMI_F32>(a.partial + team * a.cols + c, dw[v], a.cols - c);
+  }
+}
+
+template <int DT, bool W32>
+__global__ void __launch_bounds__(kBlock) norm_backward_long_kernel(NormBackwardArgs a) {
+  using E = Elem<DT>;
+  using T = typename E::type;
+  __shared__ uint32_t slots[2][kBlock / 64];
+  int turn = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
+    const T* grad = (const T*)a.grad + row * a.cols;
+    const T* h = (const T*)a.h + row * a.cols;
+    const float r = a.rstd[row];
+    float dot = 0.0f;
+    for (int64_t c = (int64_t)threadIdx.x * 8; c < a.cols; c += kBlock * 8) {
+      float fg[8], fh[8], w[8];
+      E::unpack(load_some<DT>(grad + c, a.cols - c), fg);
+      E::unpack(load_some<DT>(h + c, a.cols - c), fh);
+      Weight<DT, W32>::load(a.weight, c, a.cols, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dot = fmaf(fg[i] * w[i], fh[i] * r, dot);
+    }
+    dot = __uint_as_float(team_reduce<SumOp, kBlock>(__float_as_uint(dot), slots[turn]));
+    const float mean = dot / (float)a.cols;
+    for (int64_t c = (int64_t)threadIdx.x * 8; c < a.cols; c += kBlock * 8) {
+      float fg[8], fh[8], fm[8], w[8], d[8];
+      E::unpack(load_some<DT>(grad + c, a.cols - c), fg);
+      E::unpack(load_some<DT>(h + c, a.cols - c), fh);
+      E::unpack(a.grad_h ? load_some<DT>((const T*)a.grad_h + row * a.cols + c, a.cols - c) : E::zero(), fm);
+      Weight<DT, W32>::load(a.weight, c, a.cols, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) d[i] = fmaf(r, fg[i] * w[i] - fh[i] * r * mean, fm[i]);
+      store_some<DT>((T*)a.dx + row * a.cols + c, d, a.cols - c);
+    }
+  }
+}
+
+// Sums over rows of a stripe of columns: of x itself (NORM false), or of g h r (NORM true, the weight gradient of
+// norms whose rows do not stay in registers).  blockIdx.x is the stripe of 8 * kBlock columns, blockIdx.y takes every
+// gridDim.y-th row and leaves a partial row.
+template <int DT, bool NORM>
+__global__ void __launch_bounds__(kBlock) column_partial_kernel(const typename Elem<DT>::type* __restrict__ x, const typename Elem<DT>::type* __restrict__ h,
+                                                                const float* __restrict__ rstd, int64_t rows, int64_t cols, float* __restrict__ partial) {
+  using E = Elem<DT>;
+  const int64_t c = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * 8;
+  if (c >= cols) return;
+  float sum[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum[i] = 0.0f;
+#pragma unroll 4
+  for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
+    float f[8];
+    E::unpack(load_some<DT>(x + row * cols + c, cols - c), f);
+    if constexpr (NORM) {
+      float fh[8];
+      E::unpack(load_some<DT>(h + row * cols + c, cols - c), fh);
+      const float r = rstd[row];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] = fmaf(f[i], fh[i] * r, sum[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] += f[i];
+    }
+  }
+  store_some<OPTIMI_F32>(partial + (int64_t)blockIdx.y * cols + c, sum, cols - c);
+}
+
+// Adds the partial rows: 32 columns a workgroup, its eight groups of 32 lanes take every eighth partial row.
+template <int OUT>
+__global__ void __launch_bounds__(kBlock) column_finish_kernel(const float* __restrict__ partial, int64_t parts, int64_t cols,
+                                                               typename Elem<OUT>::type* __restrict__ out) {
+  __shared__ float sums[8][33];
+  const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
+  for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < cols; c0 += (int64_t)gridDim.x * 32) {
+    float s = 0.0f;
+    if (c0 + lane < cols) {
+#pragma unroll 8
+      for (int64_t p = group; p < parts; p += 8) s += partial[p * cols + c0 + lane];
+    }
+    sums[group][lane] = s;
+    __syncthreads();
+    if (group == 0 && c0 + lane < cols) {
+#pragma unroll
+      for (int g = 1; g < 8; ++g) s += sums[g][lane];
+      out[c0 + lane] = Elem<OUT>::put(s);
+    }
+    __syncthreads();
+  }
+}
+
+// ------------------------------------------------------------------------------------
+// Host side
+// ------------------------------------------------------------------------------------
+
+template <class F>
+int by_dtype(int dtype, F f) {
+  switch (dtype) {
+    case OPTIMI_F32: return f(std::integral_constant<int, OPTIMI_F32>{});
+    case OPTIMI_BF16: return f(std::integral_constant<int, OPTIMI_BF16>{});
+    default: return f(std::integral_constant<int, OPTIMI_F16>{});
+  }
+}
+
+// Calls f(team, vectors per lane) for rows of `cols` elements that stay in registers.
+template <class F>
+int by_width(int64_t cols, F f) {
+#define OPTIMI_WIDTH(team, vpt) \
+  if (cols <= (int64_t)8 * team * vpt) return f(std::integral_constant<int, team>{}, std::integral_constant<int, vpt>{})
+  OPTIMI_WIDTH(64, 1);
+  OPTIMI_WIDTH(64, 2);
+  static_assert(kWaveRowCols == 64 * 8 * 2, "the widest row of one wavefront");
+  OPTIMI_WIDTH(256, 1);
+  OPTIMI_WIDTH(256, 2);
+  OPTIMI_WIDTH(256, 3);
+  OPTIMI_WIDTH(256, 4);
+  OPTIMI_WIDTH(256, 6);
+  return f(std::integral_constant<int, 256>{}, std::integral_constant<int, 8>{});
+#undef OPTIMI_WIDTH
+}
+
+inline int rows_per_block(int64_t cols) { return cols <= kWaveRowCols ? kBlock / 64 : 1; }
+
+// Workgroups of a pass that ends in partial rows: enough of them to fill the machine, few enough for the partial
+// rows to be a small part of the traffic.
+constexpr int64_t kPartialBlocks = 512;
+inline int64_t partial_blocks(int64_t rows, int64_t cols) {
+  const int per = rows_per_block(cols);
+  const int64_t n = (rows + per - 1) / per;
+  return n < kPartialBlocks ? n : kPartialBlocks;
+}
+inline int64_t norm_partials(int64_t rows, int64_t cols) {
+  if (cols > kLongCols) return rows < 64 ? rows : 64;
+  return partial_blocks(rows, cols) * rows_per_block(cols);
+}
+
+int finish_columns(const float* partial, int64_t parts, int64_t cols, int dtype, void* out, hipStream_t stream) {
+  if (cols == 0) return 0;
+  return by_dtype(dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    column_finish_kernel<DT><<<dim3(blocks_for(cols, 32)), dim3(kBlock), 0, stream>>>(partial, parts, cols, (typename Elem<DT>::type*)out);
+    OPTIMI_INT8_TRY(hipGetLastError());
+    return 0;
+  });
+}
+
+}  // namespace
+
+namespace optimi_int8 {
+
+// Column sums of a [rows, cols] matrix, for bias gradients: see int8_gemm.hip.
+int64_t column_sum_workspace(int64_t rows, int64_t cols) { return (rows < 128 ? rows : 128) * cols * 4; }
+
+int column_sum(const void* x, int64_t rows, int64_t cols, int dtype, void* out, void* workspace, hipStream_t stream) {
+  if (cols == 0) return 0;
+  const int64_t parts = rows < 128 ? rows : 128;
+  return by_dtype(dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    using T = typename Elem<DT>::type;
+    const unsigned stripes = (unsigned)((cols + kBlock * 8 - 1) / (kBlock * 8));
+    if (parts > 0) {
+      column_partial_kernel<DT, false><<<dim3(stripes, (unsigned)parts), dim3(kBlock), 0, stream>>>((const T*)x, nullptr, nullptr, rows, cols, (float*)workspace);
+      OPTIMI_INT8_TRY(hipGetLastError());
+    }
+    return finish_columns((const float*)workspace, parts, cols, dtype, out, stream);
+  });
+}
+
+}  // namespace optimi_int8
+
+extern "C" {
+
+int optimi_hip_int8_quantize(const void* x, int64_t rows, int64_t cols, int dtype, int8_t* values, float* scales, optimi_stream_t stream_) {
+  if (!valid_dtype(dtype)) return OPTIMI_ERR_DTYPE;
+  if (int rc = check_shape(rows, cols)) return rc;
+  if (rows == 0) return 0;
+  if (!scales || (cols && (!x || !values))) return OPTIMI_ERR_NULL;
+  if (!aligned_to(x, elem_bytes(dtype)) || !aligned_to(scales, 4)) return OPTIMI_ERR_ALIGN;
+  hipStream_t stream = (hipStream_t)stream_;
+  return by_dtype(dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    using T = typename Elem<DT>::type;
+    if (cols > kLongCols) {
+      quantize_long_kernel<DT><<<dim3(blocks_for(rows, 1)), dim3(kBlock), 0, stream>>>((const T*)x, rows, cols, values, scales);
+    } else {
+      by_width(cols, [&](auto team, auto vpt) {
+        quantize_kernel<DT, decltype(team)::value, decltype(vpt)::value>
+            <<<dim3(blocks_for(rows, rows_per_block(cols))), dim3(kBlock), 0, stream>>>((const T*)x, rows, cols, values, scales);
+        return 0;
+      });
+    }
+    OPTIMI_INT8_TRY(hipGetLastError());
+    return 0;
+  });
+}
+
+int optimi_hip_int8_dequantize(const int8_t* values, const float* scales, int64_t rows, int64_t cols, int dtype, void* out, optimi_stream_t stream_) {
+  if (!valid_dtype(dtype)) return OPTIMI_ERR_DTYPE;
+  if (int rc = check_shape(rows, cols)) return rc;
+  if (rows == 0 || cols == 0) return 0;
+  if (!values || !scales || !out) return OPTIMI_ERR_NULL;
+  if (!aligned_to(out, elem_bytes(dtype)) || !aligned_to(scales, 4)) return OPTIMI_ERR_ALIGN;
+  int team = 1;
+  while (team < kBlock && (int64_t)team * 8 < cols) team *= 2;
+  return by_dtype(dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    dequantize_kernel<DT><<<dim3(blocks_for(rows, kBlock / team)), dim3(kBlock), 0, (hipStream_t)stream_>>>(values, scales, rows, cols, team,
+                                                                                                         (typename Elem<DT>::type*)out);
+    OPTIMI_INT8_TRY(hipGetLastError());
+    return 0;
+  });
+}
+
+int optimi_hip_add_rms_norm_int8(const void* x, const void* residual, const void* weight, int64_t rows, int64_t cols, int dtype, int weight_dtype,
+                                 double eps, void* h, int8_t* values, float* scales, float* rstd, optimi_stream_t stream_) {
+  if (!valid_dtype(dtype) || (weight_dtype != dtype && weight_dtype != OPTIMI_F32)) return OPTIMI_ERR_DTYPE;
+  if (int rc = check_shape(rows, cols)) return rc;
+  if (!(eps >= 0.0)) return OPTIMI_ERR_ARG;
+  if (rows == 0) return 0;
+  if (cols == 0) return OPTIMI_ERR_SIZE;  // the mean of no elements
+  if (!x || !weight || !values || !scales || !rstd || (residual && !h)) return OPTIMI_ERR_NULL;
+  const int64_t size = elem_bytes(dtype);
+  if (!aligned_to(x, size) || !aligned_to(residual, size) || !aligned_to(h, size) || !aligned_to(weight, elem_bytes(weight_dtype)) ||
+      !aligned_to(scales, 4) || !aligned_to(rstd, 4))
+    return OPTIMI_ERR_ALIGN;
+  hipStream_t stream = (hipStream_t)stream_;
+  const NormArgs args{x, residual, weight, rows, cols, (float)eps, h, values, scales, rstd};
+  return by_dtype(dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    auto with = [&](auto w32) {
+      constexpr bool W32 = decltype(w32)::value;
+      if (cols > kLongCols) {
+        norm_long_kernel<DT, W32><<<dim3(blocks_for(rows, 1)), dim3(kBlock), 0, stream>>>(args);
+      } else {
+        by_width(cols, [&](auto team, auto vpt) {
+          norm_kernel<DT, W32, decltype(team)::value, decltype(vpt)::value><<<dim3(blocks_for(rows, rows_per_block(cols))), dim3(kBlock), 0, stream>>>(args);
+          return 0;
+        });
+      }
+      OPTIMI_INT8_TRY(hipGetLastError());
+      return 0;
+    };
+    if (weight_dtype == dtype) return with(std::false_type{});
+    return with(std::true_type{});
+  });
+}
+
+int64_t optimi_hip_add_rms_norm_int8_backward_workspace(int64_t rows, int64_t cols) {
+  if (int rc = check_shape(rows, cols)) return rc;
+  return norm_partials(rows, cols) * cols * 4;
+}
+
+int optimi_hip_add_rms_norm_int8_backward(const void* grad, const void* grad_h, const void* h, const float* rstd, const void* weight, int64_t rows,
+                                          int64_t cols, int dtype, int weight_dtype, void* dx, void* dweight, void* workspace, optimi_stream_t stream_) {
+  if (!valid_dtype(dtype) || (weight_dtype != dtype && weight_dtype != OPTIMI_F32)) return OPTIMI_ERR_DTYPE;
+  if (int rc = check_shape(rows, cols)) return rc;
+  if (cols == 0) return OPTIMI_ERR_SIZE;
+  if (!weight || !dweight || (rows && (!grad || !h || !rstd || !dx || !workspace))) return OPTIMI_ERR_NULL;
+  const int64_t size = elem_bytes(dtype), wsize = elem_bytes(weight_dtype);
+  if (!aligned_to(grad, size) || !aligned_to(grad_h, size) || !aligned_to(h, size) || !aligned_to(dx, size) || !aligned_to(weight, wsize) ||
+      !aligned_to(dweight, wsize) || !aligned_to(rstd, 4) || !aligned_to(workspace, 4))
+    return OPTIMI_ERR_ALIGN;
+  hipStream_t stream = (hipStream_t)stream_;
+  const int64_t parts = norm_partials(rows, cols);
+  if (rows > 0) {
+    const NormBackwardArgs args{grad, grad_h, h, weight, rstd, rows, cols, dx, (float*)workspace};
+    const int rc = by_dtype(dtype, [&](auto dt) {
+      constexpr int DT = decltype(dt)::value;
+      using T = typename Elem<DT>::type;
+      auto with = [&](auto w32) {
+        constexpr bool W32 = decltype(w32)::value;
+        if (cols > kLongCols) {
+          norm_backward_long_kernel<DT, W32><<<dim3(blocks_for(rows, 1)), dim3(kBlock), 0, stream>>>(args);
+          OPTIMI_INT8_TRY(hipGetLastError());
+          const unsigned stripes = (unsigned)((cols + kBlock * 8 - 1) / (kBlock * 8));
+          column_partial_kernel<DT, true><<<dim3(stripes, (unsigned)parts), dim3(kBlock), 0, stream>>>((const T*)grad, (const T*)h, rstd, rows, cols, (float*)workspace);
+        } else {
+          by_width(cols, [&](auto team, auto vpt) {
+            norm_backward_kernel<DT, W32, decltype(team)::value, decltype(vpt)::value>
+                <<<dim3((unsigned)partial_blocks(rows, cols)), dim3(kBlock), 0, stream>>>(args);
+            return 0;
+          });
+        }
+        OPTIMI_INT8_TRY(hipGetLastError());
+        return 0;
+      };
+      if (weight_dtype == dtype) return with(std::false_type{});
+      return with(std::true_type{});
+    });
+    if (rc) return rc;
+  }
+  return finish_columns((const float*)workspace, parts, cols, weight_dtype, dweight, stream);
+}
+
+}  // extern "C"

@@ -1412,6 +1412,8 @@ py::object make_release_hook(const std::shared_ptr<ReleaseHookCore>& core) {
 
 }  // namespace
 
+void bind_int8(py::module& mod);  // int8_binding.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   mod.doc() = "PyTorch-ROCm binding of the optimi_hip C ABI";
   mod.attr("KAHAN") = (uint32_t)OPTIMI_KAHAN;
@@ -1468,4 +1470,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, mod) {
   mod.def("ranger_single", &ranger_single);
   mod.def("sgd_release", &sgd_release);
   mod.def("ranger_release", &ranger_release);
+  bind_int8(mod);
 }

@@ -1,0 +1,234 @@
+"""Training with activations held in 8 bits: the operators, the linear layer made of them, and the
+model preparation beside ``prepare_for_gradient_release``.
+
+A linear layer keeps its input for the backward pass; here it keeps it as int8 with one scale per
+row (token), half of what 16 bits take, multiplies the same int8 values with the weight's in the
+forward pass, and forms the weight gradient from them in 16 bits.  The gradient of the input
+is a plain product of the incoming gradient and the weight in their own type: gradients are not
+quantized.  The optimizers, gradient release and ``state_dict`` see ordinary parameters and
+gradients.  (No counterpart in the reference.)
+
+All functions run HIP kernels on the current stream, take float32, bfloat16 or float16 tensors of
+any number of leading dimensions (a non-contiguous one is copied first), raise ``RuntimeError`` for
+tensors they cannot take, and may be captured into HIP graphs.  Tensors that a caller brings from another
+stream are the caller's to synchronize, as everywhere in PyTorch.
+"""
+
+from __future__ import annotations
+
+import warnings
+from typing import Iterable, Sequence
+
+import torch
+from torch import Tensor, nn
+from torch.autograd.function import once_differentiable
+
+from . import backend
+
+__all__ = [
+    "int8_quantize", "int8_dequantize", "int8_matmul", "int8_weight_grad", "add_rms_norm_int8", "add_rms_norm_int8_backward",
+    "int8_linear", "add_rms_norm_int8_linear", "Int8Linear", "prepare_for_int8_linear", "remove_int8_linear",
+]
+
+
+def int8_quantize(x: Tensor) -> tuple[Tensor, Tensor]:
+    """``(values, scales)`` of the rows (last dimension) of ``x``: int8 values in [-127, 127] and one float32
+    scale per row, the smallest power of two that holds the row; ``values * scales`` stands for ``x``, at
+    most half a scale away.  Rows of zeros get the scale 1.  A row with an infinity or a NaN gets the scale NaN,
+    so that an overflow stays visible.  Not differentiable."""
+    return backend.ext().int8_quantize(x)
+
+
+def int8_dequantize(values: Tensor, scales: Tensor, dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """``values * scales[..., None]`` in ``dtype``."""
+    return backend.ext().int8_dequantize(values, scales, dtype)
+
+
+def int8_matmul(values: Tensor, scales: Tensor, weight_values: Tensor, weight_scales: Tensor, bias: Tensor | None = None,
+                dtype: torch.dtype = torch.bfloat16) -> Tensor:
+    """``(values * scales[..., None]) @ (weight_values * weight_scales[:, None]).T + bias`` in ``dtype``, from int8
+    ``values [..., K]`` and ``weight_values [N, K]``; the sums are exact in int32 (K <= 131071)."""
+    return backend.ext().int8_matmul(values, scales, weight_values, weight_scales, bias, dtype)
+
+
+def int8_weight_grad(grad: Tensor, values: Tensor, scales: Tensor, bias: bool = False):
+    """The weight gradient ``grad.T @ (values * scales[..., None])`` (``[N, K]``, grad's dtype) of a linear layer
+    from its incoming gradient ``grad [..., N]`` and the int8 checkpoint of its input ``[..., K]``, summed in
+    float32; with ``bias`` also the bias gradient, as ``(weight_grad, bias_grad)``."""
+    dw, db = backend.ext().int8_weight_grad(grad, values, scales, bias)
+    return (dw, db) if bias else dw
+
+
+def add_rms_norm_int8(x: Tensor, weight: Tensor, residual: Tensor | None = None, eps: float = 1e-6) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    """``(values, scales, h, rstd)``: the sum ``h = x + residual`` (``x`` itself without a residual), its
+    ``rstd = 1 / sqrt(mean(h**2) + eps)`` per row, and the int8 form of ``h * rstd * weight``, which is
+    never written in more bits.  ``weight`` has x's dtype or float32.  Not differentiable by itself: see
+    ``add_rms_norm_int8_linear`` and ``add_rms_norm_int8_backward``."""
+    return backend.ext().add_rms_norm_int8(x, weight, residual, eps)
+
+
+def add_rms_norm_int8_backward(grad: Tensor, h: Tensor, rstd: Tensor, weight: Tensor, grad_h: Tensor | None = None) -> tuple[Tensor, Tensor]:
+    """``(dx, dweight)`` of the norm for the gradient ``grad`` of its output; ``dx`` is the gradient of ``x`` and of
+    ``residual`` alike and contains ``grad_h``, what arrives at ``h`` itself."""
+    return backend.ext().add_rms_norm_int8_backward(grad, h, rstd, weight, grad_h)
+
+
+def _check_linear(x: Tensor, weight: Tensor, bias: Tensor | None):
+    backend.check_supported(weight)
+    if x.dtype != weight.dtype or (bias is not None and bias.dtype != weight.dtype):
+        raise TypeError(f"optimi_amd: an int8 linear layer needs input, weight and bias of one dtype, got {x.dtype}, {weight.dtype}"
+                        + (f" and {bias.dtype}" if bias is not None else ""))
+
+
+def _product(values, scales, weight, bias, dtype):
+    weight_values, weight_scales = int8_quantize(weight)
+    return int8_matmul(values, scales, weight_values, weight_scales, bias, dtype)
+
+
+class _Int8Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        values, scales = int8_quantize(x)
+        keep = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]  # without them the checkpoint is not needed
+        ctx.save_for_backward(weight, *((values, scales) if keep else (None, None)))
+        return _product(values, scales, weight, bias, x.dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        weight, values, scales = ctx.saved_tensors
+        dx = grad.matmul(weight) if ctx.needs_input_grad[0] else None
+        dw = db = None
+        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
+            dw, db = backend.ext().int8_weight_grad(grad, values, scales, ctx.needs_input_grad[2])
+        return dx, dw if ctx.needs_input_grad[1] else None, db
+
+
+def int8_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None) -> Tensor:
+    """``x @ weight.T + bias`` with x and weight quantized to int8 by rows, differentiable.  The backward pass
+    keeps x in 8 bits; quantization passes gradients straight through."""
+    _check_linear(x, weight, bias)
+    return _Int8Linear.apply(x, weight, bias)
+
+
+class _AddRmsNormInt8Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, norm_weight, eps, *layers):
+        weights, biases = layers[: len(layers) // 2], layers[len(layers) // 2:]
+        values, scales, h, rstd = add_rms_norm_int8(x, norm_weight, residual, eps)
+        ctx.set_materialize_grads(False)
+        ctx.with_residual = residual is not None
+        ctx.save_for_backward(values, scales, h, rstd, norm_weight, *weights)
+        outs = tuple(_product(values, scales, w, b, x.dtype) for w, b in zip(weights, biases))
+        return (h, *outs) if ctx.with_residual else outs
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, *grads):
+        values, scales, h, rstd, norm_weight, *weights = ctx.saved_tensors
+        grad_h, grads = (grads[0], grads[1:]) if ctx.with_residual else (None, grads)
+        n = len(weights)
+        need_x, need_residual, need_norm = ctx.needs_input_grad[:3]
+        dws, dbs, dy = [None] * n, [None] * n, None
+        for i, (grad, weight) in enumerate(zip(grads, weights)):
+            if grad is None:
+                continue
+            if need_x or need_residual or need_norm:
+                grad2, dy2 = grad.reshape(-1, weight.shape[0]), None if dy is None else dy.reshape(-1, weight.shape[1])
+                dy = (grad2.mm(weight) if dy2 is None else torch.addmm(dy2, grad2, weight)).reshape(h.shape)
+            need_w, need_b = ctx.needs_input_grad[4 + i], ctx.needs_input_grad[4 + n + i]
+            if need_w or need_b:
+                dw, dbs[i] = backend.ext().int8_weight_grad(grad, values, scales, need_b)
+                dws[i] = dw if need_w else None
+        dx, dnorm = grad_h, None
+        if dy is not None:
+            dx, dnorm = add_rms_norm_int8_backward(dy, h, rstd, norm_weight, grad_h)
+        return (dx if need_x else None, dx if need_residual else None, dnorm if need_norm else None, None, *dws, *dbs)
+
+
+def add_rms_norm_int8_linear(x: Tensor, norm_weight: Tensor, weights: Sequence[Tensor], biases: Sequence[Tensor | None] | None = None,
+                             residual: Tensor | None = None, eps: float = 1e-6) -> tuple[tuple[Tensor, ...], Tensor]:
+    """``(outputs, h)``: ``h = x + residual`` (``x`` itself without a residual) and, for every weight, the int8 linear
+    layer of ``rms_norm(h) * norm_weight``, differentiable.  The normed activation exists as int8 only: one checkpoint
+    that all the layers (query, key and value, or gate and up) multiply and all their weight gradients read."""
+    weights = tuple(weights)
+    biases = (None,) * len(weights) if biases is None else tuple(biases)
+    if not weights or len(biases) != len(weights):
+        raise ValueError(f"optimi_amd: got {len(weights)} weights and {len(biases)} biases")
+    for w, b in zip(weights, biases):
+        _check_linear(x, w, b)
+    outs = _AddRmsNormInt8Linear.apply(x, residual, norm_weight, eps, *weights, *biases)
+    return (outs, x) if residual is None else (outs[1:], outs[0])
+
+
+class Int8Linear(nn.Linear):
+    """``nn.Linear`` computed by ``int8_linear``; parameters and ``state_dict`` are nn.Linear's."""
+
+    def forward(self, x: Tensor) -> Tensor:
+        return int8_linear(x, self.weight, self.bias)
+
+
+def _has_hooks(module: nn.Module) -> bool:
+    return bool(module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks)
+
+
+def _is_norm_of(norm: nn.Module, layer: nn.Module) -> bool:
+    return (type(norm) is nn.RMSNorm and type(layer) is Int8Linear and norm.elementwise_affine
+            and tuple(norm.normalized_shape) == (layer.in_features,) and not _has_hooks(norm) and not _has_hooks(layer))
+
+
+class _Int8Sequential(nn.Sequential):
+    """Runs an RMSNorm that is directly followed by an Int8Linear as one node."""
+
+    def forward(self, x):
+        modules = list(self)
+        i = 0
+        while i < len(modules):
+            if i + 1 < len(modules) and _is_norm_of(modules[i], modules[i + 1]):
+                norm, layer = modules[i], modules[i + 1]
+                eps = torch.finfo(x.dtype).eps if norm.eps is None else norm.eps
+                (x,), _ = add_rms_norm_int8_linear(x, norm.weight, [layer.weight], [layer.bias], eps=eps)
+                i += 2
+            else:
+                x = modules[i](x)
+                i += 1
+        return x
+
+
+_PREPARED = {nn.Linear: Int8Linear, nn.Sequential: _Int8Sequential}
+_MODULES_ATTR = "_int8_linear_modules"
+
+
+def prepare_for_int8_linear(model: nn.Module, skip: Iterable[str] = ()) -> nn.Module:
+    """Makes every ``nn.Linear`` of ``model`` (in place; itself included) an ``Int8Linear``, except those whose qualified
+    name contains one of the strings in ``skip``, and lets an ``nn.RMSNorm`` directly before one in an ``nn.Sequential``
+    hand it int8 values.  Subclasses of these modules are left alone.  Parameters stay the same objects: optimizers
+    built before or after, gradient release and checkpoints work as they did.  ``ValueError`` if the model is prepared
+    already or holds no such layer.  Undo with ``remove_int8_linear``."""
+    if isinstance(skip, str):
+        skip = (skip,)
+    skip = tuple(skip)
+    if hasattr(model, _MODULES_ATTR):
+        raise ValueError("`model` is prepared for int8 linear layers already.")
+    layers = [m for name, m in model.named_modules() if type(m) is nn.Linear and not any(s in name for s in skip)]
+    if not layers:
+        raise ValueError("`model` has no `nn.Linear` to compute in int8.")
+    changed = layers + [m for m in model.modules() if type(m) is nn.Sequential]
+    for module in changed:
+        module.__class__ = _PREPARED[type(module)]
+    object.__setattr__(model, _MODULES_ATTR, changed)
+    return model
+
+
+def remove_int8_linear(model: nn.Module) -> nn.Module:
+    """Gives the layers that ``prepare_for_int8_linear`` changed their former classes; warns if there are none."""
+    changed = getattr(model, _MODULES_ATTR, None)
+    if changed is None:
+        warnings.warn("`model` has no int8 linear layers to remove.")
+        return model
+    back = {new: old for old, new in _PREPARED.items()}
+    for module in changed:
+        if type(module) in back:
+            module.__class__ = back[type(module)]
+    object.__delattr__(model, _MODULES_ATTR)
+    return model
