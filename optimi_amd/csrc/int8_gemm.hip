@@ -69,6 +69,7 @@ __device__ __forceinline__ void run_steps(int begin, int end, Fetch fetch, Fetch
     fetch(step, p0);
     settle(p0);
     fetch(++step, p1);
+    __builtin_amdgcn_sched_barrier(0);
     multiply(p0);
     settle(p1);
   } else {
@@ -77,13 +78,16 @@ __device__ __forceinline__ void run_steps(int begin, int end, Fetch fetch, Fetch
   }
   for (; step + 2 < end; step += 2) {
     fetch(step + 1, p0);
+    __builtin_amdgcn_sched_barrier(0);  // the loads start before the products do; left alone, they are moved behind them
     multiply(p1);
     settle(p0);
     fetch(step + 2, p1);
+    __builtin_amdgcn_sched_barrier(0);
     multiply(p0);
     settle(p1);
   }
   fetch_last(end - 1, p0);
+  __builtin_amdgcn_sched_barrier(0);
   multiply(p1);
   settle(p0);
   multiply_last(p0);
@@ -145,8 +149,9 @@ __device__ __forceinline__ i32x4 first_bytes(int n) {
   return v;
 }
 
-// A tile of R rows of kStep bytes in LDS.  16-byte piece c of row r lies at piece c ^ (r & 7): the eight rows that
-// eight neighbouring lanes read at the same k then lie in eight different groups of banks.
+// A tile of R rows of kStep bytes in LDS.  16-byte piece c of row r lies at piece c ^ (r / 2 mod 8).  LDS serves 256
+// bytes a cycle, two rows: of the 16 rows that 16 neighbouring lanes read at the same k, the even ones lie in one half of
+// the banks and the odd ones in the other, each in eight different places.
 constexpr int kStep = 128;
 template <int R, int THREADS>
 struct ByteTile {
@@ -155,7 +160,7 @@ struct ByteTile {
   static __device__ __forceinline__ void where(int i, int& row, int& piece) {
     const int p = i * THREADS + threadIdx.x;
     row = p / 8;
-    piece = (p % 8) ^ (row & 7);
+    piece = (p % 8) ^ (row / 2 & 7);
   }
   // rows from the buffer's start on, `len` bytes long each, from byte k0 on; a piece behind a row's end is the next row's
   static __device__ __forceinline__ void copy(Buffer src, uint32_t len, uint32_t k0, int8_t* lds) {
@@ -188,7 +193,7 @@ struct ByteTile {
     for (int i = 0; i < kPieces; ++i) *(u32x4*)(lds + (i * THREADS + threadIdx.x) * 16) = v[i];
   }
   // the 16 bytes of row r from piece c on
-  static __device__ __forceinline__ i32x4 read(const int8_t* lds, int r, int c) { return *(const i32x4*)(lds + r * kStep + ((c ^ (r & 7)) * 16)); }
+  static __device__ __forceinline__ i32x4 read(const int8_t* lds, int r, int c) { return *(const i32x4*)(lds + r * kStep + ((c ^ (r / 2 & 7)) * 16)); }
 };
 
 // Tiles of BM x BN, WM x WN wavefronts, each with BM/WM x BN/WN of it in registers as 32 x 32 blocks of sums.  The
@@ -246,23 +251,28 @@ __global__ void __launch_bounds__(WM * WN * 64) matmul_kernel(MatmulArgs p) {
   // `left`: bytes of the sum that are left; what lies behind them in the tiles is not part of it
   const int left = end == all ? (int)(p.k - (int64_t)(all - 1) * kStep) : kStep;
   auto multiply_some = [&](const int8_t* a, const int8_t* b, auto last) {
-#pragma unroll
-    for (int ks = 0; ks < kStep / 32; ++ks) {
-      i32x4 fa[kM], fb[kN];
+    i32x4 fa[2][kM], fb[2][kN];
+    auto read = [&](int ks, i32x4 (&ra)[kM], i32x4 (&rb)[kN]) {
 #pragma unroll
       for (int j = 0; j < kN; ++j) {
-        fb[j] = TB::read(b, wn + j * 32 + lane % 32, ks * 2 + lane / 32);
-        if (last.value && (ks + 1) * 32 > left) fb[j] &= first_bytes(left - ks * 32 - lane / 32 * 16);
+        rb[j] = TB::read(b, wn + j * 32 + lane % 32, ks * 2 + lane / 32);
+        if (last.value && (ks + 1) * 32 > left) rb[j] &= first_bytes(left - ks * 32 - lane / 32 * 16);
       }
 #pragma unroll
-      for (int i = 0; i < kM; ++i) fa[i] = TA::read(a, wm + i * 32 + lane % 32, ks * 2 + lane / 32);
+      for (int i = 0; i < kM; ++i) ra[i] = TA::read(a, wm + i * 32 + lane % 32, ks * 2 + lane / 32);
+    };
+    read(0, fa[0], fb[0]);
+#pragma unroll
+    for (int ks = 0; ks < kStep / 32; ++ks) {  // the next reads are on their way while this slice multiplies
+      if (ks + 1 < kStep / 32) read(ks + 1, fa[(ks + 1) % 2], fb[(ks + 1) % 2]);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < kM; ++i)
 #pragma unroll
-        for (int j = 0; j < kN; ++j) acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[j], fa[i], acc[j][i], 0, 0, 0);
+        for (int j = 0; j < kN; ++j) acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[ks % 2][j], fa[ks % 2][i], acc[j][i], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
-
   run_steps(begin, end, fetch, fetch_last, settle, [&](auto which) { multiply_some(which.value ? a1 : a0, which.value ? b1 : b0, std::false_type{}); },
             [&](auto which) { multiply_some(which.value ? a1 : a0, which.value ? b1 : b0, std::true_type{}); });
 
@@ -603,6 +613,219 @@ __global__ void __launch_bounds__(WN * WC * 64) weight_grad_kernel(WeightGradArg
   }
 }
 
+// The same for large 16-bit products, where all that counts is that the matrix instructions never wait: 256 x 256 tiles, 64
+// rows a step, two pairs of tiles in LDS, eight wavefronts with 128 x 64 sums each.  Gradients go to LDS past the registers;
+// the values have to become 16-bit numbers on the way, and are loaded two steps ahead, so that the conversion of the next
+// step's values can be spread over this step's products without waiting for memory.  outs is a multiple of 8, grad aligned to
+// 16 bytes, and there are 16 values at least.
+template <int DT>
+__global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p) {
+  using T = typename Elem<DT>::type;
+  using P = Product<DT>;
+  constexpr int kTile = 256, kRows = 64, kN = 8, kC = 4, kPieces = 2;
+  using H = HalfTile<kTile>;
+  __shared__ __attribute__((aligned(1024))) short g0[kRows * kTile], g1[kRows * kTile], q0[kRows * kTile], q1[kRows * kTile];
+  const int tn = (int)((p.outs + kTile - 1) / kTile), tc = (int)((p.cols + kTile - 1) / kTile);
+  const int split = blockIdx.x / (tn * tc);
+  const Tile tile = tile_of(blockIdx.x % (tn * tc), tn, tc);
+  const int64_t n0 = (int64_t)tile.row * kTile, c0 = (int64_t)tile.col * kTile;
+  const int wave = wave_id(), lane = threadIdx.x % 64;
+  const int wn = wave / 4 * 128, wc = wave % 4 * 64;
+  const int all = (int)((p.rows + kRows - 1) / kRows);
+  const int begin = split * p.steps_per_split, end = begin + p.steps_per_split < all ? begin + p.steps_per_split : all;
+
+  f32x4 acc[kN][kC];
+#pragma unroll
+  for (int i = 0; i < kN; ++i)
+#pragma unroll
+    for (int j = 0; j < kC; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+
+  // Gradients: a wave's copy fills two rows of LDS; the sources follow the swizzle.  Columns behind the matrix come from the
+  // next row (or not at all, behind the last) and end in sums that are not stored.
+  const int outs = (int)(p.outs - n0 < kTile ? p.outs - n0 : kTile);
+  auto copy = [&](int step, short* g) {
+    const int64_t m0 = (int64_t)step * kRows;
+    const int rows = (int)(p.rows - m0 < kRows ? p.rows - m0 : kRows);
+    const Buffer from = buffer_of((const T*)p.grad + m0 * p.outs + n0, ((int64_t)(rows - 1) * p.outs + outs) * 2);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int place = i * 512 + threadIdx.x;
+      const int row = place / 32, in = place % 32;
+      const int n = H::at(row, in / 2) - row * kTile + in % 2 * 8;
+      copy16_to_lds(from, ((uint32_t)row * (uint32_t)p.outs + n) * 2, g + (i * 512 + wave * 64) * 8);
+    }
+  };
+  // Values: a lane has 16 neighbours of two rows.  Rows behind the last are the last one again, under a scale of 0;
+  // columns behind the matrix are never used.  A piece that would run over the end of all values is loaded from a little
+  // before, and shifted into its place when it is converted.
+  const int64_t total = p.rows * p.cols;
+  const int at_row = threadIdx.x / 16, at_col = threadIdx.x % 16;
+  const uint32_t col = (uint32_t)c0 + (c0 + at_col * 16 < p.cols ? at_col * 16 : 0);
+  u32x4 vq[2][kPieces];
+  float sq[2][kPieces];
+  auto place_of = [&](int step, int i, int64_t& start, uint32_t& limit) {
+    const int64_t m0 = (int64_t)step * kRows, first = m0 * p.cols;
+    start = first < total - 16 ? first : total - 16;
+    const int64_t left = total - 16 - start;
+    limit = (uint32_t)(left < 0x7fffffff ? left : 0x7fffffff);
+    const int rows = (int)(p.rows - m0 < kRows ? p.rows - m0 : kRows), row = at_row + i * 32;
+    return (uint32_t)(row < rows ? row : rows - 1) * (uint32_t)p.cols + col + (uint32_t)(first - start);
+  };
+  auto load = [&](int step, u32x4 (&v)[kPieces], float (&s)[kPieces]) {
+    const int64_t m0 = (int64_t)step * kRows;
+    const int rows = (int)(p.rows - m0 < kRows ? p.rows - m0 : kRows);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      int64_t start;
+      uint32_t limit;
+      const uint32_t at = place_of(step, i, start, limit);
+      v[i] = *(const u32x4_align1*)(p.values + start + (at < limit ? at : limit));
+      const int row = at_row + i * 32;
+      s[i] = p.scales[m0 + (row < rows ? row : rows - 1)];
+    }
+  };
+  auto shift = [&](int step, u32x4 (&v)[kPieces], float (&s)[kPieces]) {  // the very last step only
+    const int rows = (int)(p.rows - (int64_t)step * kRows);
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+      int64_t start;
+      uint32_t limit;
+      const uint32_t at = place_of(step, i, start, limit), by = at > limit ? (at - limit) * 8 : 0;
+      uint64_t lo = (uint64_t)v[i][1] << 32 | v[i][0], hi = (uint64_t)v[i][3] << 32 | v[i][2];
+      if (by >= 64) {
+        lo = hi >> (by - 64 & 63);
+        hi = 0;
+      } else if (by > 0) {
+        lo = lo >> by | hi << (64 - by);
+        hi >>= by;
+      }
+      v[i] = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+      if (at_row + i * 32 >= rows) s[i] = 0.0f;
+    }
+  };
+  // Four values as 16-bit numbers: bytes as unsigned numbers are 128 too large, (u - 128) s has one rounding, and none
+  // under a power of two.
+  auto convert = [&](uint32_t word, float s) {
+    const uint32_t u = word ^ 0x80808080u;
+    const float minus = -128.0f * s;
+    float f[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = fmaf((float)((u >> (8 * e)) & 0xffu), s, minus);
+    return u32x2{P::pair(f[0], f[1]), P::pair(f[2], f[3])};
+  };
+  auto write_half = [&](int half, const u32x4 (&v)[kPieces], const float (&s)[kPieces], short* q) {  // eight values of piece half / 2
+    const int i = half / 2;
+    const u32x2 a = convert(v[i][half % 2 * 2], s[i]), b = convert(v[i][half % 2 * 2 + 1], s[i]);
+    *(u32x4*)(q + H::at(at_row + i * 32, at_col) + half % 2 * 8) = u32x4{a[0], a[1], b[0], b[1]};
+  };
+
+  // Where a lane's part of 16 columns lies: chunks differ in five address bits only, so chunk i of the wave's is one
+  // exclusive or away from its first.  The addresses are formed anew for every step: kept over the loop, they would take more
+  // registers than there are.
+  typedef OPTIMI_LDS s16x4* Ptr;
+  auto column = [&](const short* t, int first, int i, int ks) {
+    const char* from = (const char*)t + (first ^ (i * 32)) + ks * 32 * kTile * 2;
+    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)from);
+    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(from + 16 * kTile * 2));
+    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  auto anew = [](int v) {
+    asm volatile("" : "+v"(v));
+    return v & 0x7fff;
+  };
+  const int first_g = (H::at(lane / 4, wn / 16) + lane % 4 * 4) * 2, first_q = (H::at(lane / 4, wc / 16) + lane % 4 * 4) * 2;
+  const int left = end == all ? (int)(p.rows - (int64_t)(all - 1) * kRows) : kRows;
+  // One step's products in sixteen groups; a group's operands are read two groups earlier, and four of the groups are followed
+  // by a quarter of the next step's conversion.
+  auto multiply = [&](const short* g, const short* q, auto last, const u32x4 (&v)[kPieces], const float (&s)[kPieces], short* next) {
+    const int at_g = anew(first_g), at_q = anew(first_q);
+    s16x8 fq[2][kC], fg[3];
+    auto keep = [&](s16x8 f, int ks) {  // copied gradients of rows behind the last are whatever was in LDS, infinities maybe
+      if (!last.value) return f;
+      s16x8 mask;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) mask[e] = ks * 32 + e / 4 * 16 + lane / 16 * 4 + e % 4 < left ? -1 : 0;
+      return f & mask;
+    };
+#pragma unroll
+    for (int j = 0; j < kC; ++j) fq[0][j] = column(q, at_q, j, 0);
+    fg[0] = column(g, at_g, 0, 0);
+    fg[1] = column(g, at_g, 1, 0);
+#pragma unroll
+    for (int t = 0; t < 2 * kN; ++t) {
+      const int ks = t / kN, i = t % kN;
+      if (t + 2 < 2 * kN) fg[(t + 2) % 3] = column(g, at_g, (t + 2) % kN, (t + 2) / kN);
+      if (t == 3) {
+#pragma unroll
+        for (int j = 0; j < kC; ++j) fq[1][j] = column(q, at_q, j, 1);
+      }
+      const s16x8 f = keep(fg[t % 3], ks);
+#pragma unroll
+      for (int j = 0; j < kC; ++j) acc[i][j] = P::mfma(fq[ks][j], f, acc[i][j]);
+      if (!last.value && t % 3 == 1 && t / 3 < 2 * kPieces) write_half(t / 3, v, s, next);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto step_on = [&](int step, auto which) {
+    constexpr int W = decltype(which)::value;
+    copy(step + 1, W ? g0 : g1);
+    if (step + 2 < end) load(step + 2, vq[W], sq[W]);
+    if (step + 2 == all) shift(step + 1, vq[1 - W], sq[1 - W]);
+    __builtin_amdgcn_sched_barrier(0);  // the loads start before the products do; left alone, they are moved behind them
+    multiply(W ? g1 : g0, W ? q1 : q0, std::false_type{}, vq[1 - W], sq[1 - W], W ? q0 : q1);
+    __syncthreads();
+  };
+  auto start = [&](int step, auto which) {
+    constexpr int W = decltype(which)::value;
+    copy(step, W ? g1 : g0);
+    load(step, vq[W], sq[W]);
+    if (step + 1 < end) load(step + 1, vq[1 - W], sq[1 - W]);
+    if (step + 1 == all) shift(step, vq[W], sq[W]);
+#pragma unroll
+    for (int half = 0; half < 2 * kPieces; ++half) write_half(half, vq[W], sq[W], W ? q1 : q0);
+    __syncthreads();
+  };
+
+  // the last step works on the first pair of tiles
+  if (begin < end) {
+    int step = begin;
+    if ((end - begin) % 2) {
+      start(step, Pair<0>{});
+    } else {
+      start(step, Pair<1>{});
+      step_on(step++, Pair<1>{});
+    }
+    for (; step + 1 < end; step += 2) {
+      step_on(step, Pair<0>{});
+      step_on(step + 1, Pair<1>{});
+    }
+    multiply(g0, q0, std::true_type{}, vq[0], sq[0], q1);
+  }
+
+  using O = OutBlock<16, 64>;
+  uint32_t* block = (uint32_t*)((char*)(wave < 4 ? g1 : q1) + wave % 4 * O::kBytes);
+  const int64_t c = c0 + wc + O::col();
+  const int64_t some = p.cols - c;
+#pragma unroll
+  for (int i = 0; i < kN; ++i) {
+#pragma unroll
+    for (int j = 0; j < kC; ++j) O::put(block, lane % 16, j * 4 + lane / 16, __builtin_bit_cast(u32x4, acc[i][j]));
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int t = 0; t < O::kTurns; ++t) {
+      const int64_t n = n0 + wn + i * 16 + O::row(t);
+      uint32_t v[8];
+      O::get(block, O::row(t), v);
+      const float(&f)[8] = reinterpret_cast<const float(&)[8]>(v);
+      if (n < p.outs && some > 0) {
+        if (p.splits > 1) store_some<OPTIMI_F32>(p.partial + ((int64_t)split * p.outs + n) * p.cols + c, f, some);
+        else store_some<DT>((T*)p.out + n * p.cols + c, f, some);
+      }
+    }
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
 // Adds the splits' sums, always in the same order.
 template <int DT>
 __global__ void __launch_bounds__(256) weight_grad_finish_kernel(WeightGradArgs p) {
@@ -748,7 +971,7 @@ int optimi_hip_int8_weight_grad(const void* grad, const int8_t* values, const fl
     } else {
       const bool direct = outs % 8 == 0 && aligned_to(grad, 16);
       if (c.tile == 256) {
-        if (direct) weight_grad_kernel<DT, 256, 256, 2, 4, 64, true><<<grid, dim3(512), 0, stream>>>(args);
+        if (direct) weight_grad_wide_kernel<DT><<<grid, dim3(512), 0, stream>>>(args);
         else weight_grad_kernel<DT, 256, 256, 2, 4, 64, false><<<grid, dim3(512), 0, stream>>>(args);
       } else {
         if (direct) weight_grad_kernel<DT, 128, 128, 2, 2, 64, true><<<grid, dim3(256), 0, stream>>>(args);

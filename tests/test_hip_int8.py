@@ -113,6 +113,24 @@ def test_matmul(hip_device, shape, dtype):
         R.close(y, want, allowed, f"{shape} bias={bias is not None}")
 
 
+# products of so many tiles that the largest ones are used: even and odd widths, sums that end inside a step, one step alone
+LARGE = [(2900, 2830, 272), (2817, 3000, 1111), (3000, 2900, 100), (5000, 1700, 128), (2600, 3400, 1), (4096, 4097, 640)]
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES, ids=R.IDS)
+@pytest.mark.parametrize("shape", LARGE, ids=lambda s: "x".join(map(str, s)))
+def test_large_matmul(hip_device, shape, dtype):
+    m, n, k = shape
+    a, sa, b, sb = (t.to(hip_device) for t in int8_inputs(m, n, k, 11, False))
+    bias = rand((n,), dtype, 5).to(hip_device)
+    y = optimi.int8_matmul(a, sa, b, sb, bias=bias, dtype=dtype)
+    want, allowed = R.matmul(a, sa, b, sb, bias, dtype)
+    R.close(y, want.cpu(), allowed.cpu(), str(shape))
+    if k > 1:
+        y = optimi.int8_matmul(misaligned(a, hip_device), sa, misaligned(b, hip_device), sb, bias=bias, dtype=dtype)
+        R.close(y, want.cpu(), allowed.cpu(), f"{shape} off the grid")
+
+
 @pytest.mark.parametrize("shape", [(1, 40, 512), (20, 70, 96), (130, 300, 256), (300, 260, 1024)], ids=lambda s: "x".join(map(str, s)))
 def test_matmul_takes_views_and_any_alignment(hip_device, shape):
     m, n, k = shape
@@ -174,6 +192,35 @@ def test_weight_grad(hip_device, shape, dtype):
         R.close(db, *R.column_sum(g, dtype), f"bias {shape}")
         alone = optimi.int8_weight_grad(g.to(hip_device), q.to(hip_device), s.to(hip_device))
         assert alone.dtype == dtype and torch.equal(alone, dw), "the same bits on every run"
+
+
+LARGE_GRADS = [(1, 3000, 2900), (64, 2904, 2831), (65, 3000, 2800), (129, 2817, 3000), (200, 2896, 2817), (257, 5000, 1700), (1000, 33000, 16), (70, 33000, 3), (500, 16, 33001), (5, 7, 50000)]
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES, ids=R.IDS)
+@pytest.mark.parametrize("shape", LARGE_GRADS, ids=lambda s: "x".join(map(str, s)))
+def test_large_weight_grad(hip_device, shape, dtype):
+    rows, outs, cols = shape
+    g = rand((rows, outs), dtype, 3, 1e-2).to(hip_device)
+    q, s = (t.to(hip_device) for t in checkpoint(rows, cols, 4))
+    want, allowed = R.weight_grad(g, q, s, dtype)
+    R.close(optimi.int8_weight_grad(g, q, s), want.cpu(), allowed.cpu(), str(shape))
+    R.close(optimi.int8_weight_grad(misaligned(g, hip_device), misaligned(q, hip_device), s), want.cpu(), allowed.cpu(), f"{shape} off the grid")
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES, ids=R.IDS)
+@pytest.mark.parametrize("shape", [(65, 3000, 2800), (130, 2904, 2831)], ids=lambda s: "x".join(map(str, s)))
+def test_large_weight_grad_of_gradients_that_are_not_finite(hip_device, shape, dtype):
+    rows, outs, cols = shape
+    g = rand((rows, outs), dtype, 4, 1e-2).to(hip_device)
+    q, s = (t.to(hip_device) for t in checkpoint(rows, cols, 5))
+    q[q == 0] = 1
+    g[rows - 1, 5], g[0, 9], g[rows // 2, outs - 1] = float("inf"), float("-inf"), float("nan")
+    for _ in range(2):  # the second time LDS holds the first's infinities
+        got, want = optimi.int8_weight_grad(g, q, s).double(), R.weight_grad(g, q, s, dtype)[0]
+        assert torch.equal(torch.isnan(got), torch.isnan(want))
+        inf = torch.isinf(want)
+        assert torch.equal(torch.isinf(got), inf) and torch.equal(got[inf], want[inf])
 
 
 @pytest.mark.parametrize("dtype", R.DTYPES, ids=R.IDS)
