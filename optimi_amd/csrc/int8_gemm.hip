@@ -26,6 +26,13 @@ __device__ __forceinline__ void copy16_to_lds(Buffer from, uint32_t offset, void
   __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (OPTIMI_LDS void*)lds, 16, offset, 0, 0, 0);
 }
 
+// All of this wave's copies and loads are done, and everybody's are: said outright, since a copy to LDS is an access to
+// memory that a barrier by itself does not wait for.
+__device__ __forceinline__ void meet() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)threadIdx.x / 64); }
 
 // Consecutive workgroups go to the eight XCDs in turn, and each XCD has an L2 of its own.  An XCD gets a contiguous
@@ -196,70 +203,54 @@ struct ByteTile {
   static __device__ __forceinline__ i32x4 read(const int8_t* lds, int r, int c) { return *(const i32x4*)(lds + r * kStep + ((c ^ (r / 2 & 7)) * 16)); }
 };
 
-// Tiles of BM x BN, WM x WN wavefronts, each with BM/WM x BN/WN of it in registers as 32 x 32 blocks of sums.  The
-// weight's rows are the matrix instruction's first operand: a lane then holds four neighbouring channels of a row.
-template <int DT, int BM, int BN, int WM, int WN, bool ALIGNED>
-__global__ void __launch_bounds__(WM * WN * 64) matmul_kernel(MatmulArgs p) {
-  constexpr int kWaves = WM * WN, kThreads = kWaves * 64, kM = BM / WM / 32, kN = BN / WN / 32;
+// What every tile of the product shares: where it lies, one step's products, and the way out.
+template <int DT, int BM, int BN, int WM, int WN>
+struct MatmulTile {
+  static constexpr int kWaves = WM * WN, kThreads = kWaves * 64, kM = BM / WM / 32, kN = BN / WN / 32;
   using TA = ByteTile<BM, kThreads>;
   using TB = ByteTile<BN, kThreads>;
-  __shared__ __attribute__((aligned(1024))) int8_t a0[BM * kStep], a1[BM * kStep], b0[BN * kStep], b1[BN * kStep];
-  const int tm = (int)((p.m + BM - 1) / BM), tn = (int)((p.n + BN - 1) / BN);
-  const int split = blockIdx.x / (tm * tn);
-  const Tile tile = tile_of(blockIdx.x % (tm * tn), tm, tn);
-  const int64_t m0 = (int64_t)tile.row * BM, n0 = (int64_t)tile.col * BN;
-  const int wave = wave_id(), lane = threadIdx.x % 64;
-  const int wm = wave / WN * (BM / WM), wn = wave % WN * (BN / WN);
-  const int all = (int)((p.k + kStep - 1) / kStep);
-  const int begin = split * p.steps_per_split, end = begin + p.steps_per_split < all ? begin + p.steps_per_split : all;
-
+  const MatmulArgs& p;
+  int64_t m0, n0;
+  int split, begin, end, left, wave, lane, wm, wn;
+  // The weight's rows are the matrix instruction's first operand: a lane then holds four neighbouring channels of a row.
   i32x16 acc[kN][kM];
-#pragma unroll
-  for (int j = 0; j < kN; ++j)
-#pragma unroll
-    for (int i = 0; i < kM; ++i) acc[j][i] = i32x16{};
 
-  u32x4 va[TA::kPieces], vb[TB::kPieces];
-  const Buffer ra = buffer_of(p.a + m0 * p.k, (p.m - m0 < BM ? p.m - m0 : BM) * p.k), rb = buffer_of(p.b + n0 * p.k, (p.n - n0 < BN ? p.n - n0 : BN) * p.k);
-  const int8_t *pa = p.a + m0 * p.k, *pb = p.b + n0 * p.k;
-  const int rows_a = (int)(p.m - m0 < BM ? p.m - m0 : BM), rows_b = (int)(p.n - n0 < BN ? p.n - n0 : BN);
-  const uint32_t len = (uint32_t)p.k;
-  auto fetch = [&](int step, auto which) {
-    if constexpr (ALIGNED) {
-      TA::copy(ra, len, step * kStep, which.value ? a1 : a0);
-      TB::copy(rb, len, step * kStep, which.value ? b1 : b0);
-    } else {
-      TA::load(pa, rows_a, len, step * kStep, va);
-      TB::load(pb, rows_b, len, step * kStep, vb);
-    }
-  };
-  auto fetch_last = [&](int step, auto which) {
-    if constexpr (ALIGNED) {
-      fetch(step, which);
-    } else {
-      TA::load_last(pa, rows_a, len, step * kStep, va);
-      TB::load_last(pb, rows_b, len, step * kStep, vb);
-    }
-  };
-  auto settle = [&](auto which) {
-    if constexpr (!ALIGNED) {
-      TA::store(va, which.value ? a1 : a0);
-      TB::store(vb, which.value ? b1 : b0);
-    }
-    __syncthreads();
-  };
-  // `left`: bytes of the sum that are left; what lies behind them in the tiles is not part of it
-  const int left = end == all ? (int)(p.k - (int64_t)(all - 1) * kStep) : kStep;
-  auto multiply_some = [&](const int8_t* a, const int8_t* b, auto last) {
+  __device__ __forceinline__ MatmulTile(const MatmulArgs& args) : p(args) {
+    const int tm = (int)((p.m + BM - 1) / BM), tn = (int)((p.n + BN - 1) / BN);
+    split = blockIdx.x / (tm * tn);
+    const Tile tile = tile_of(blockIdx.x % (tm * tn), tm, tn);
+    m0 = (int64_t)tile.row * BM;
+    n0 = (int64_t)tile.col * BN;
+    wave = wave_id();
+    lane = threadIdx.x % 64;
+    wm = wave / WN * (BM / WM);
+    wn = wave % WN * (BN / WN);
+    const int all = (int)((p.k + kStep - 1) / kStep);
+    begin = split * p.steps_per_split;
+    end = begin + p.steps_per_split < all ? begin + p.steps_per_split : all;
+    left = end == all ? (int)(p.k - (int64_t)(all - 1) * kStep) : kStep;  // bytes of the last step that belong to the sum
+#pragma unroll
+    for (int j = 0; j < kN; ++j)
+#pragma unroll
+      for (int i = 0; i < kM; ++i) acc[j][i] = i32x16{};
+  }
+  __device__ __forceinline__ const int8_t* a() const { return p.a + m0 * p.k; }
+  __device__ __forceinline__ const int8_t* b() const { return p.b + n0 * p.k; }
+  __device__ __forceinline__ int rows_a() const { return (int)(p.m - m0 < BM ? p.m - m0 : BM); }
+  __device__ __forceinline__ int rows_b() const { return (int)(p.n - n0 < BN ? p.n - n0 : BN); }
+
+  // what lies behind the sum's end in the last step's tiles is left out
+  template <bool LAST>
+  __device__ __forceinline__ void multiply(const int8_t* ta, const int8_t* tb) {
     i32x4 fa[2][kM], fb[2][kN];
-    auto read = [&](int ks, i32x4 (&ra)[kM], i32x4 (&rb)[kN]) {
+    auto read = [&](int ks, i32x4(&ra)[kM], i32x4(&rb)[kN]) {
 #pragma unroll
       for (int j = 0; j < kN; ++j) {
-        rb[j] = TB::read(b, wn + j * 32 + lane % 32, ks * 2 + lane / 32);
-        if (last.value && (ks + 1) * 32 > left) rb[j] &= first_bytes(left - ks * 32 - lane / 32 * 16);
+        rb[j] = TB::read(tb, wn + j * 32 + lane % 32, ks * 2 + lane / 32);
+        if (LAST && (ks + 1) * 32 > left) rb[j] &= first_bytes(left - ks * 32 - lane / 32 * 16);
       }
 #pragma unroll
-      for (int i = 0; i < kM; ++i) ra[i] = TA::read(a, wm + i * 32 + lane % 32, ks * 2 + lane / 32);
+      for (int i = 0; i < kM; ++i) ra[i] = TA::read(ta, wm + i * 32 + lane % 32, ks * 2 + lane / 32);
     };
     read(0, fa[0], fb[0]);
 #pragma unroll
@@ -272,76 +263,288 @@ __global__ void __launch_bounds__(WM * WN * 64) matmul_kernel(MatmulArgs p) {
         for (int j = 0; j < kN; ++j) acc[j][i] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fb[ks % 2][j], fa[ks % 2][i], acc[j][i], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
-  };
-  run_steps(begin, end, fetch, fetch_last, settle, [&](auto which) { multiply_some(which.value ? a1 : a0, which.value ? b1 : b0, std::false_type{}); },
-            [&](auto which) { multiply_some(which.value ? a1 : a0, which.value ? b1 : b0, std::true_type{}); });
-
-  // The sums go through LDS (the second pair of tiles, which nobody reads any more) 32 rows at a time, so that a
-  // lane has eight neighbouring channels to scale and to store.
-  using E = Elem<DT>;
-  using T = typename E::type;
-  using O = OutBlock<32, BN / WN>;
-  static_assert(kWaves / 2 * O::kBytes <= BM * kStep && kWaves / 2 * O::kBytes <= BN * kStep, "half of the waves' blocks fit either tile");
-  uint32_t* block = (uint32_t*)((wave < kWaves / 2 ? a1 : b1) + wave % (kWaves / 2) * O::kBytes);
-  const int64_t n = n0 + wn + O::col();
-  const int64_t some = p.n - n;
-  float sb[8], bias[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    sb[e] = e < some && p.splits == 1 ? p.b_scales[n + e] : 0.0f;
-    bias[e] = e < some && p.splits == 1 && p.bias ? E::get(((const T*)p.bias)[n + e]) : 0.0f;
   }
+
+  // The sums go through LDS 32 rows at a time, so that a lane has eight neighbouring channels to scale and to store.
+  using O = OutBlock<32, BN / WN>;
+  __device__ __forceinline__ void store(uint32_t* block) {
+    using E = Elem<DT>;
+    using T = typename E::type;
+    const int64_t n = n0 + wn + O::col();
+    const int64_t some = p.n - n;
+    float sb[8], bias[8];
 #pragma unroll
-  for (int i = 0; i < kM; ++i) {
+    for (int e = 0; e < 8; ++e) {
+      sb[e] = e < some && p.splits == 1 ? p.b_scales[n + e] : 0.0f;
+      bias[e] = e < some && p.splits == 1 && p.bias ? E::get(((const T*)p.bias)[n + e]) : 0.0f;
+    }
 #pragma unroll
-    for (int j = 0; j < kN; ++j)
+    for (int i = 0; i < kM; ++i) {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const u32x4 v{(uint32_t)acc[j][i][q * 4], (uint32_t)acc[j][i][q * 4 + 1], (uint32_t)acc[j][i][q * 4 + 2], (uint32_t)acc[j][i][q * 4 + 3]};
-        O::put(block, lane % 32, j * 8 + q * 2 + lane / 32, v);
-      }
-    __builtin_amdgcn_wave_barrier();
+      for (int j = 0; j < kN; ++j)
 #pragma unroll
-    for (int t = 0; t < O::kTurns; ++t) {
-      const int64_t m = m0 + wm + i * 32 + O::row(t);
-      uint32_t v[8];
-      O::get(block, O::row(t), v);
-      if (m < p.m && some > 0) {
-        if (p.splits > 1) {
-          store_some<OPTIMI_F32>((float*)p.partial + ((int64_t)split * p.m + m) * p.n + n, reinterpret_cast<const float(&)[8]>(v), some);
-        } else {
-          const float sa = p.a_scales[m];
-          float f[8];
+        for (int q = 0; q < 4; ++q) {
+          const u32x4 v{(uint32_t)acc[j][i][q * 4], (uint32_t)acc[j][i][q * 4 + 1], (uint32_t)acc[j][i][q * 4 + 2], (uint32_t)acc[j][i][q * 4 + 3]};
+          O::put(block, lane % 32, j * 8 + q * 2 + lane / 32, v);
+        }
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] = fmaf((float)(int32_t)v[e] * sa, sb[e], bias[e]);
-          store_some<DT>((T*)p.out + m * p.n + n, f, some);
+      for (int t = 0; t < O::kTurns; ++t) {
+        const int64_t m = m0 + wm + i * 32 + O::row(t);
+        uint32_t v[8];
+        O::get(block, O::row(t), v);
+        if (m < p.m && some > 0) {
+          if (p.splits > 1) {
+            store_some<OPTIMI_F32>((float*)p.partial + ((int64_t)split * p.m + m) * p.n + n, reinterpret_cast<const float(&)[8]>(v), some);
+          } else {
+            const float sa = p.a_scales[m];
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = fmaf((float)(int32_t)v[e] * sa, sb[e], bias[e]);
+            store_some<DT>((T*)p.out + m * p.n + n, f, some);
+          }
         }
       }
+      __builtin_amdgcn_wave_barrier();
     }
-    __builtin_amdgcn_wave_barrier();
+  }
+};
+
+// Two pairs of tiles in LDS.  ALIGNED: rows start on 16 bytes.
+template <int DT, int BM, int BN, int WM, int WN, bool ALIGNED>
+__global__ void __launch_bounds__(WM * WN * 64) matmul_kernel(MatmulArgs p) {
+  using M = MatmulTile<DT, BM, BN, WM, WN>;
+  using TA = typename M::TA;
+  using TB = typename M::TB;
+  __shared__ __attribute__((aligned(1024))) int8_t a0[BM * kStep], a1[BM * kStep], b0[BN * kStep], b1[BN * kStep];
+  M tile(p);
+  u32x4 va[TA::kPieces], vb[TB::kPieces];
+  const int rows_a = tile.rows_a(), rows_b = tile.rows_b();
+  const uint32_t len = (uint32_t)p.k;
+  const Buffer ra = buffer_of(tile.a(), rows_a * p.k), rb = buffer_of(tile.b(), rows_b * p.k);
+  auto fetch = [&](int step, auto which) {
+    if constexpr (ALIGNED) {
+      TA::copy(ra, len, step * kStep, which.value ? a1 : a0);
+      TB::copy(rb, len, step * kStep, which.value ? b1 : b0);
+    } else {
+      TA::load(tile.a(), rows_a, len, step * kStep, va);
+      TB::load(tile.b(), rows_b, len, step * kStep, vb);
+    }
+  };
+  auto fetch_last = [&](int step, auto which) {
+    if constexpr (ALIGNED) {
+      fetch(step, which);
+    } else {
+      TA::load_last(tile.a(), rows_a, len, step * kStep, va);
+      TB::load_last(tile.b(), rows_b, len, step * kStep, vb);
+    }
+  };
+  auto settle = [&](auto which) {
+    if constexpr (!ALIGNED) {
+      TA::store(va, which.value ? a1 : a0);
+      TB::store(vb, which.value ? b1 : b0);
+    }
+    meet();
+  };
+  run_steps(tile.begin, tile.end, fetch, fetch_last, settle,
+            [&](auto which) { tile.template multiply<false>(which.value ? a1 : a0, which.value ? b1 : b0); },
+            [&](auto which) { tile.template multiply<true>(which.value ? a1 : a0, which.value ? b1 : b0); });
+  // the second pair of tiles is free
+  static_assert(M::kWaves / 2 * M::O::kBytes <= BM * kStep && M::kWaves / 2 * M::O::kBytes <= BN * kStep, "half of the waves' blocks fit either tile");
+  tile.store((uint32_t*)((tile.wave < M::kWaves / 2 ? a1 : b1) + tile.wave % (M::kWaves / 2) * M::O::kBytes));
+}
+
+// Small tiles, for products with less work than the machine has places: a workgroup is alone on its CU or nearly, and
+// what counts is that a step does not take a trip to memory.  Four pairs of tiles, three steps on their way.
+template <int DT, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(WM * WN * 64) matmul_deep_kernel(MatmulArgs p) {
+  using M = MatmulTile<DT, BM, BN, WM, WN>;
+  using TA = typename M::TA;
+  using TB = typename M::TB;
+  __shared__ __attribute__((aligned(1024))) int8_t a0[BM * kStep], a1[BM * kStep], a2[BM * kStep], a3[BM * kStep];
+  __shared__ __attribute__((aligned(1024))) int8_t b0[BN * kStep], b1[BN * kStep], b2[BN * kStep], b3[BN * kStep];
+  M tile(p);
+  const uint32_t len = (uint32_t)p.k;
+  const Buffer ra = buffer_of(tile.a(), tile.rows_a() * p.k), rb = buffer_of(tile.b(), tile.rows_b() * p.k);
+  // Steps behind the end are fetched as well, so that the number of copies on their way is always the same; their
+  // addresses lie outside of the buffers and nothing is read.
+  auto fetch = [&](int step, int8_t* a, int8_t* b) {
+    const uint32_t k0 = step < tile.end ? (uint32_t)step * kStep : 0x40000000u;
+    TA::copy(ra, len, k0, a);
+    TB::copy(rb, len, k0, b);
+  };
+  // This wave's copies but those of the two youngest steps have landed, then everybody's have; the step before is read.
+  auto meet_early = [&]() {
+    constexpr int kYoung = 2 * (TA::kPieces + TB::kPieces);
+    static_assert(kYoung == 8, "the count in the instruction below");
+    asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  };
+  const int begin = tile.begin, end = tile.end;
+  if (begin < end) {
+    fetch(begin, a0, b0);
+    fetch(begin + 1, a1, b1);
+    fetch(begin + 2, a2, b2);
+    auto one = [&](int at, int8_t* a, int8_t* b, int8_t* next_a, int8_t* next_b, auto last) {
+      meet_early();
+      fetch(at + 3, next_a, next_b);
+      __builtin_amdgcn_sched_barrier(0);
+      tile.template multiply<last.value>(a, b);
+    };
+    // rounds of four steps without a branch (the compiler counts the copies in flight by itself too, and a branch makes it
+    // wait for more of them than it has to), then the last one to four
+    int step = begin;
+    for (; step + 4 < end; step += 4) {
+      one(step, a0, b0, a3, b3, std::false_type{});
+      one(step + 1, a1, b1, a0, b0, std::false_type{});
+      one(step + 2, a2, b2, a1, b1, std::false_type{});
+      one(step + 3, a3, b3, a2, b2, std::false_type{});
+    }
+    const int more = end - step;
+    if (more > 1) {
+      one(step, a0, b0, a3, b3, std::false_type{});
+      if (more > 2) {
+        one(step + 1, a1, b1, a0, b0, std::false_type{});
+        if (more > 3) {
+          one(step + 2, a2, b2, a1, b1, std::false_type{});
+          one(step + 3, a3, b3, a2, b2, std::true_type{});
+        } else {
+          one(step + 2, a2, b2, a1, b1, std::true_type{});
+        }
+      } else {
+        one(step + 1, a1, b1, a0, b0, std::true_type{});
+      }
+    } else {
+      one(step, a0, b0, a3, b3, std::true_type{});
+    }
+  }
+  meet();  // all copies have landed and all tiles are read
+  static_assert(M::kWaves * M::O::kBytes <= 2 * BM * kStep && M::kWaves / 2 * M::O::kBytes <= BM * kStep, "half of the waves' blocks fit a tile");
+  tile.store((uint32_t*)((tile.wave < M::kWaves / 2 ? a0 : a1) + tile.wave % (M::kWaves / 2) * M::O::kBytes));
+}
+
+// A few rows against a weight: the weight is read once and nothing else counts.  A wavefront takes kRowsB rows of it, 16
+// bytes a lane, multiplies them with up to M rows of the activation, and adds up over its lanes at the end.  KSPLIT
+// wavefronts share the same rows of the weight, each a part of the sum, where there are few of them.
+constexpr int kRowsB = 4;
+struct IntSum {
+  static __device__ __forceinline__ uint32_t join(uint32_t a, uint32_t b) { return a + b; }
+};
+template <int DT, int M, int KSPLIT>
+__global__ void __launch_bounds__(256) matvec_kernel(MatmulArgs p) {
+  using E = Elem<DT>;
+  using T = typename E::type;
+  __shared__ int32_t sums[KSPLIT > 1 ? 4 : 1][kRowsB * M];
+  const int wave = wave_id(), lane = threadIdx.x % 64, part = wave % KSPLIT;
+  const int64_t n0 = ((int64_t)blockIdx.x * (4 / KSPLIT) + wave / KSPLIT) * kRowsB;
+  int32_t acc[kRowsB][M];
+#pragma unroll
+  for (int r = 0; r < kRowsB; ++r)
+#pragma unroll
+    for (int m = 0; m < M; ++m) acc[r][m] = 0;
+  const int8_t* row[kRowsB];
+#pragma unroll
+  for (int r = 0; r < kRowsB; ++r) row[r] = p.b + (n0 + r < p.n ? n0 + r : p.n - 1) * p.k;  // rows behind the last: the last again
+  auto some = [&](int64_t k, auto whole) {
+    u32x4 w[kRowsB], x[M];
+#pragma unroll
+    for (int r = 0; r < kRowsB; ++r) w[r] = whole.value ? *(const u32x4_align1*)(row[r] + k) : load_bytes(row[r], k, p.k);
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+      const int8_t* a = p.a + (m < p.m ? m : p.m - 1) * p.k;
+      x[m] = whole.value ? *(const u32x4_align1*)(a + k) : load_bytes(a, k, p.k);
+    }
+#pragma unroll
+    for (int r = 0; r < kRowsB; ++r)
+#pragma unroll
+      for (int m = 0; m < M; ++m)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[r][m] = __builtin_amdgcn_sdot4((int)w[r][i], (int)x[m][i], acc[r][m], false);
+  };
+  int64_t k = (int64_t)part * 1024 + lane * 16;
+#pragma unroll 2
+  for (; k + 16 <= p.k; k += KSPLIT * 1024) some(k, std::true_type{});
+  if (k < p.k) some(k, std::false_type{});
+#pragma unroll
+  for (int r = 0; r < kRowsB; ++r)
+#pragma unroll
+    for (int m = 0; m < M; ++m) acc[r][m] = (int32_t)wave_reduce<IntSum>((uint32_t)acc[r][m]);
+  if constexpr (KSPLIT > 1) {
+    if (lane == 0) {
+#pragma unroll
+      for (int r = 0; r < kRowsB; ++r)
+#pragma unroll
+        for (int m = 0; m < M; ++m) sums[wave][r * M + m] = acc[r][m];
+    }
+    __syncthreads();
+    if (part != 0) return;
+  }
+  // lane r * M + m stores result (m, n0 + r)
+  if (lane >= kRowsB * M) return;
+  int32_t sum = 0;
+  if constexpr (KSPLIT > 1) {
+#pragma unroll
+    for (int w = 0; w < KSPLIT; ++w) sum += sums[wave + w][lane];
+  } else {
+#pragma unroll
+    for (int r = 0; r < kRowsB; ++r)
+#pragma unroll
+      for (int m = 0; m < M; ++m) sum = lane == r * M + m ? acc[r][m] : sum;
+  }
+  const int64_t m = lane % M, n = n0 + lane / M;
+  if (m >= p.m || n >= p.n) return;
+  const float bias = p.bias ? E::get(((const T*)p.bias)[n]) : 0.0f;
+  ((T*)p.out)[m * p.n + n] = E::put(fmaf((float)sum * p.a_scales[m], p.b_scales[n], bias));
+}
+
+// Copies of up to two matrices whose rows of `from` bytes lie `to` bytes apart afterwards, a multiple of 16, with zeros in between: what
+// the asynchronous copies need.
+struct PadArgs {
+  const int8_t* src[2];
+  int64_t rows[2];
+  uint32_t from, to;
+  int8_t* dst;  // the second matrix behind the first
+};
+__global__ void __launch_bounds__(256) pad_kernel(PadArgs p) {
+  const uint32_t pieces = p.to / 16;
+  for (int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / 64; row < p.rows[0] + p.rows[1]; row += (int64_t)gridDim.x * 4) {
+    const int8_t* src = row < p.rows[0] ? p.src[0] + row * p.from : p.src[1] + (row - p.rows[0]) * p.from;
+    for (uint32_t c = threadIdx.x % 64; c < pieces; c += 64) *(u32x4*)(p.dst + row * p.to + c * 16) = load_bytes(src, c * 16, p.from);
   }
 }
 
-// Adds the splits' whole-number sums, four columns a lane.
+// Adds the splits' whole-number sums, four neighbours a lane.
 template <int DT>
 __global__ void __launch_bounds__(256) matmul_finish_kernel(MatmulArgs p) {
   using E = Elem<DT>;
   using T = typename E::type;
-  for (int64_t m = blockIdx.y; m < p.m; m += gridDim.y) {
-    const int64_t n = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (n >= p.n) continue;
+  const int64_t all = p.m * p.n;
+  for (int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; at < all; at += (int64_t)gridDim.x * 1024) {
+    typedef i32x4 i32x4_align4 __attribute__((aligned(4)));
+    const int some = (int)(all - at < 4 ? all - at : 4);
     int32_t sum[4] = {0, 0, 0, 0};
-    for (int s = 0; s < p.splits; ++s) {
-      const int32_t* from = p.partial + ((int64_t)s * p.m + m) * p.n + n;
+    if (some == 4) {
+#pragma unroll 4
+      for (int s = 0; s < p.splits; ++s) {
+        const i32x4 v = *(const i32x4_align4*)(p.partial + s * all + at);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (n + e < p.n) sum[e] += from[e];
+        for (int e = 0; e < 4; ++e) sum[e] += v[e];
+      }
+    } else {
+      for (int s = 0; s < p.splits; ++s)
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (e < some) sum[e] += p.partial[s * all + at + e];
     }
+    int64_t m = at / p.n, n = at % p.n;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      if (n + e >= p.n) continue;
-      const float bias = p.bias ? E::get(((const T*)p.bias)[n + e]) : 0.0f;
-      ((T*)p.out)[m * p.n + n + e] = E::put(fmaf((float)sum[e] * p.a_scales[m], p.b_scales[n + e], bias));
+      if (e >= some) break;
+      const float bias = p.bias ? E::get(((const T*)p.bias)[n]) : 0.0f;
+      ((T*)p.out)[at + e] = E::put(fmaf((float)sum[e] * p.a_scales[m], p.b_scales[n], bias));
+      if (++n == p.n) {
+        n = 0;
+        ++m;
+      }
     }
   }
 }
@@ -352,6 +555,7 @@ __global__ void __launch_bounds__(256) matmul_finish_kernel(MatmulArgs p) {
 
 struct WeightGradArgs {
   const void* grad;
+  int64_t stride;      // of the gradient's rows, in elements
   const int8_t* values;
   const float* scales;
   int64_t rows, outs, cols;
@@ -440,13 +644,13 @@ __global__ void __launch_bounds__(WN * WC * 64) weight_grad_kernel(WeightGradArg
   float sq[kQ];
   const int outs = (int)(p.outs - n0 < BN ? p.outs - n0 : BN), cols = (int)(p.cols - c0 < BC ? p.cols - c0 : BC);
   auto copy = [&](int64_t m0, int rows, short* g) {  // LDS place -> row, place in row; the source follows the swizzle
-    const Buffer from = buffer_of((const T*)p.grad + m0 * p.outs + n0, ((int64_t)(rows - 1) * p.outs + outs) * 2);
+    const Buffer from = buffer_of((const T*)p.grad + m0 * p.stride + n0, ((int64_t)(rows - 1) * p.stride + outs) * 2);
 #pragma unroll
     for (int i = 0; i < kGrad; ++i) {
       const int place = i * kThreads + threadIdx.x;
       const int row = place / (BN / 8), in = place % (BN / 8);
       const int n = TG::at(row, in / 2) - row * BN + in % 2 * 8;
-      copy16_to_lds(from, ((uint32_t)row * (uint32_t)p.outs + n) * 2, g + (i * kThreads + wave * 64) * 8);
+      copy16_to_lds(from, ((uint32_t)row * (uint32_t)p.stride + n) * 2, g + (i * kThreads + wave * 64) * 8);
     }
   };
   // A full step's loads.  Columns behind the matrix are read from its first ones and never used; a piece that begins inside
@@ -547,7 +751,7 @@ __global__ void __launch_bounds__(WN * WC * 64) weight_grad_kernel(WeightGradArg
       *(u32x4*)to = v[0];
       *(u32x4*)(to + 8) = v[1];
     }
-    __syncthreads();
+    meet();
   };
   // rows 32 ks .. 32 ks + 31 of 16 columns, as the matrix instruction takes them (in an order of rows that is the same for both operands)
   auto column = [&](const short* t, int pitch, int offset, int ks) {
@@ -642,17 +846,17 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
 
   // Gradients: a wave's copy fills two rows of LDS; the sources follow the swizzle.  Columns behind the matrix come from the
   // next row (or not at all, behind the last) and end in sums that are not stored.
-  const int outs = (int)(p.outs - n0 < kTile ? p.outs - n0 : kTile);
+  const int width = (int)(p.stride - n0 < kTile ? p.stride - n0 : kTile);
   auto copy = [&](int step, short* g) {
     const int64_t m0 = (int64_t)step * kRows;
     const int rows = (int)(p.rows - m0 < kRows ? p.rows - m0 : kRows);
-    const Buffer from = buffer_of((const T*)p.grad + m0 * p.outs + n0, ((int64_t)(rows - 1) * p.outs + outs) * 2);
+    const Buffer from = buffer_of((const T*)p.grad + m0 * p.stride + n0, ((int64_t)(rows - 1) * p.stride + width) * 2);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int place = i * 512 + threadIdx.x;
       const int row = place / 32, in = place % 32;
       const int n = H::at(row, in / 2) - row * kTile + in % 2 * 8;
-      copy16_to_lds(from, ((uint32_t)row * (uint32_t)p.outs + n) * 2, g + (i * 512 + wave * 64) * 8);
+      copy16_to_lds(from, ((uint32_t)row * (uint32_t)p.stride + n) * 2, g + (i * 512 + wave * 64) * 8);
     }
   };
   // Values: a lane has 16 neighbours of two rows.  Rows behind the last are the last one again, under a scale of 0;
@@ -773,7 +977,7 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
     if (step + 2 == all) shift(step + 1, vq[1 - W], sq[1 - W]);
     __builtin_amdgcn_sched_barrier(0);  // the loads start before the products do; left alone, they are moved behind them
     multiply(W ? g1 : g0, W ? q1 : q0, std::false_type{}, vq[1 - W], sq[1 - W], W ? q0 : q1);
-    __syncthreads();
+    meet();
   };
   auto start = [&](int step, auto which) {
     constexpr int W = decltype(which)::value;
@@ -783,7 +987,7 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
     if (step + 1 == all) shift(step, vq[W], sq[W]);
 #pragma unroll
     for (int half = 0; half < 2 * kPieces; ++half) write_half(half, vq[W], sq[W], W ? q1 : q0);
-    __syncthreads();
+    meet();
   };
 
   // the last step works on the first pair of tiles
@@ -860,27 +1064,104 @@ struct Cut {
   int tile;
   int64_t tiles;
   int splits, steps_per_split;
+  void split(int64_t steps, int64_t parts) {
+    splits = parts > 1 ? (int)parts : 1;
+    steps_per_split = (int)((steps + splits - 1) / splits);
+    if (splits > 1) splits = (int)((steps + steps_per_split - 1) / steps_per_split);
+  }
 };
 constexpr int kCus = 256;
-Cut cut(int64_t rows, int64_t cols, int64_t steps, int large, int small) {
+inline int64_t tiles_of(int64_t rows, int64_t cols, int tile) { return ((rows + tile - 1) / tile) * ((cols + tile - 1) / tile); }
+
+Cut matmul_cut(int64_t m, int64_t n, int64_t k) {
+  const int64_t steps = (k + kStep - 1) / kStep;
+  const int64_t t256 = tiles_of(m, n, 256), t128 = tiles_of(m, n, 128), t64 = tiles_of(m, n, 64);
+  const double c256 = t256 <= kCus / 2 ? 1.55 : 2.05 * (double)((t256 + kCus - 1) / kCus);
+  const double c128 = t128 <= kCus / 2 ? 0.68 : t128 <= kCus ? 0.82 : 1.2 * (double)((t128 + 2 * kCus - 1) / (2 * kCus));
+  const double c64 = t64 <= kCus ? 0.25 : 0.05 + 0.22 * (double)t64 / kCus;
   Cut c;
-  auto tiles = [&](int t) { return ((rows + t - 1) / t) * ((cols + t - 1) / t); };
-  c.tile = tiles(large) >= kCus / 2 ? large : small;
-  c.tiles = tiles(c.tile);
-  c.splits = 1;
-  if (c.tiles < kCus) {
-    int64_t s = kCus / c.tiles;
-    if (s > steps / 4) s = steps / 4;
-    if (s > 16) s = 16;
-    if (s > 1) c.splits = (int)s;
-  }
-  c.steps_per_split = (int)((steps + c.splits - 1) / c.splits);
-  if (c.splits > 1) c.splits = (int)((steps + c.steps_per_split - 1) / c.steps_per_split);
+  c.tile = c256 <= c128 && c256 <= c64 ? 256 : c128 <= c64 ? 128 : 64;
+  c.tiles = c.tile == 256 ? t256 : c.tile == 128 ? t128 : t64;
+  int64_t parts = 1;
+  if (c.tile == 64 && c.tiles < kCus) parts = kCus / c.tiles < steps / 8 ? kCus / c.tiles : steps / 8;
+  c.split(steps, parts < 16 ? parts : 16);
   return c;
 }
-Cut matmul_cut(int64_t m, int64_t n, int64_t k) { return cut(m, n, (k + kStep - 1) / kStep, 256, 64); }
 Cut weight_grad_cut(int64_t rows, int64_t outs, int64_t cols, int dtype) {
-  return dtype == OPTIMI_F32 || outs < 8 || cols < 16 ? cut(outs, cols, (rows + 31) / 32, 128, 128) : cut(outs, cols, (rows + 63) / 64, 256, 128);
+  const bool narrow = outs < 8 || cols < 16;
+  const int64_t steps = dtype == OPTIMI_F32 || narrow ? (rows + 31) / 32 : (rows + 63) / 64;
+  Cut c;
+  c.tile = dtype != OPTIMI_F32 && !narrow && tiles_of(outs, cols, 256) >= kCus / 2 && rows * cols >= 16 ? 256 : 128;
+  c.tiles = tiles_of(outs, cols, c.tile);
+  int64_t parts = 1;
+  if (c.tiles < kCus) parts = kCus / c.tiles < steps / 4 ? kCus / c.tiles : steps / 4;
+  c.split(steps, parts < 16 ? parts : 16);
+  return c;
+}
+
+// Products of at most this many rows are read off the weight without tiles.
+constexpr int64_t kMostVec = 8;
+// Bytes that padded copies of the operands take, for rows that do not start on 16 bytes in tiles that are copied asynchronously.
+inline int64_t padded(int64_t bytes) { return (bytes + 15) / 16 * 16; }
+
+// What a product of these sizes does: computed alike by the call and by its workspace function.
+struct MatmulPlan {
+  bool vec;         // read off the weight
+  bool pad;         // padded copies of both operands come first
+  Cut cut;
+  int64_t pad_bytes, partial_bytes;
+};
+MatmulPlan matmul_plan(int64_t m, int64_t n, int64_t k) {
+  MatmulPlan plan{};
+  plan.vec = m <= kMostVec;
+  if (plan.vec) return plan;
+  plan.cut = matmul_cut(m, n, k);
+  plan.pad = k % 16 != 0 && plan.cut.tile > 64;
+  plan.pad_bytes = plan.pad ? (m + n) * padded(k) : 0;
+  plan.partial_bytes = plan.cut.splits > 1 ? plan.cut.splits * m * n * 4 : 0;
+  return plan;
+}
+
+struct WeightGradPlan {
+  bool pad;  // a padded copy of the gradient comes first
+  Cut cut;
+  int64_t pad_bytes, partial_bytes, bias_bytes;
+};
+WeightGradPlan weight_grad_plan(int64_t rows, int64_t outs, int64_t cols, int dtype, bool with_bias) {
+  WeightGradPlan plan{};
+  plan.bias_bytes = with_bias ? padded(column_sum_workspace(rows, outs)) : 0;
+  if (cols == 0) return plan;
+  plan.cut = weight_grad_cut(rows, outs, cols, dtype);
+  plan.pad = plan.cut.tile == 256 && outs % 8 != 0;
+  plan.pad_bytes = plan.pad ? rows * padded(outs * 2) : 0;
+  plan.partial_bytes = plan.cut.splits > 1 ? padded(plan.cut.splits * outs * cols * 4) : 0;
+  return plan;
+}
+
+template <int DT>
+int launch_vec(const MatmulArgs& args, hipStream_t stream) {
+  const bool share = (args.n + 15) / 16 < 2 * kCus && args.k > 1024;
+  const int64_t blocks = share ? (args.n + 3) / 4 : (args.n + 15) / 16;
+  const dim3 grid((unsigned)blocks), block(256);
+  auto go = [&](auto m) {
+    constexpr int M = decltype(m)::value;
+    if (share) matvec_kernel<DT, M, 4><<<grid, block, 0, stream>>>(args);
+    else matvec_kernel<DT, M, 1><<<grid, block, 0, stream>>>(args);
+  };
+  if (args.m == 1) go(Pair<1>{});
+  else if (args.m == 2) go(Pair<2>{});
+  else if (args.m <= 4) go(Pair<4>{});
+  else go(Pair<8>{});
+  OPTIMI_INT8_TRY(hipGetLastError());
+  return 0;
+}
+
+int pad_rows(const void* a, int64_t rows_a, const void* b, int64_t rows_b, int64_t from, void* dst, hipStream_t stream) {
+  const int64_t blocks = (rows_a + rows_b + 3) / 4;
+  const PadArgs args{{(const int8_t*)a, (const int8_t*)b}, {rows_a, rows_b}, (uint32_t)from, (uint32_t)padded(from), (int8_t*)dst};
+  pad_kernel<<<dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, stream>>>(args);
+  OPTIMI_INT8_TRY(hipGetLastError());
+  return 0;
 }
 
 }  // namespace
@@ -891,8 +1172,8 @@ int64_t optimi_hip_int8_matmul_workspace(int64_t m, int64_t n, int64_t k) {
   if (int rc = check_shape(m, n)) return rc;
   if (k < 0 || k > kMostSum) return OPTIMI_ERR_SIZE;
   if (m == 0 || n == 0) return 0;
-  const Cut c = matmul_cut(m, n, k);
-  return c.splits > 1 ? c.splits * m * n * 4 : 0;
+  const MatmulPlan plan = matmul_plan(m, n, k);
+  return plan.pad_bytes + plan.partial_bytes;
 }
 
 int optimi_hip_int8_matmul(const int8_t* a, const float* a_scales, const int8_t* b, const float* b_scales, const void* bias, int64_t m, int64_t n,
@@ -903,41 +1184,60 @@ int optimi_hip_int8_matmul(const int8_t* a, const float* a_scales, const int8_t*
   if (m == 0 || n == 0) return 0;
   if (!a_scales || !b_scales || !out || (k && (!a || !b))) return OPTIMI_ERR_NULL;
   const int64_t size = elem_bytes(dtype);
-  if (!aligned_to(a_scales, 4) || !aligned_to(b_scales, 4) || !aligned_to(bias, size) || !aligned_to(out, size) || !aligned_to(workspace, 4)) return OPTIMI_ERR_ALIGN;
-  const Cut c = matmul_cut(m, n, k);
-  if (c.tiles * c.splits > kMostTiles) return OPTIMI_ERR_SIZE;
-  if (c.splits > 1 && !workspace) return OPTIMI_ERR_NULL;
+  if (!aligned_to(a_scales, 4) || !aligned_to(b_scales, 4) || !aligned_to(bias, size) || !aligned_to(out, size) || !aligned_to(workspace, 16)) return OPTIMI_ERR_ALIGN;
+  const MatmulPlan plan = matmul_plan(m, n, k);
+  if (plan.pad_bytes + plan.partial_bytes > 0 && !workspace) return OPTIMI_ERR_NULL;
   hipStream_t stream = (hipStream_t)stream_;
-  const MatmulArgs args{a, a_scales, b, b_scales, bias, m, n, k, out, (int32_t*)workspace, c.splits, c.steps_per_split};
-  const bool aligned = k % 16 == 0 && aligned_to(a, 16) && aligned_to(b, 16);
+  MatmulArgs args{a, a_scales, b, b_scales, bias, m, n, k, out, nullptr, 1, 0};
+  if (plan.vec) return by_dtype(dtype, [&](auto dt) { return launch_vec<decltype(dt)::value>(args, stream); });
+
+  Cut c = plan.cut;
+  if (plan.pad) {
+    int8_t* pa = (int8_t*)workspace;
+    int8_t* pb = pa + m * padded(k);
+    if (int rc = pad_rows(a, m, b, n, k, pa, stream)) return rc;
+    args.a = pa;
+    args.b = pb;
+    args.k = padded(k);
+  }
+  const bool aligned = args.k % 16 == 0 && aligned_to(args.a, 16) && aligned_to(args.b, 16);
+  if (!aligned && c.tile > 64) {  // operands that start off the grid: tiles that go through registers are small ones
+    c.tile = 64;
+    c.tiles = tiles_of(m, n, 64);
+  }
+  if (c.tiles * c.splits > kMostTiles) return OPTIMI_ERR_SIZE;
+  args.partial = (int32_t*)((int8_t*)workspace + plan.pad_bytes);
+  args.splits = c.splits;
+  args.steps_per_split = c.steps_per_split;
   return by_dtype(dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     const dim3 grid((unsigned)(c.tiles * c.splits));
     if (c.tile == 256) {
-      if (aligned) matmul_kernel<DT, 256, 256, 2, 4, true><<<grid, dim3(512), 0, stream>>>(args);
-      else matmul_kernel<DT, 256, 256, 2, 4, false><<<grid, dim3(512), 0, stream>>>(args);
+      matmul_kernel<DT, 256, 256, 2, 4, true><<<grid, dim3(512), 0, stream>>>(args);
+    } else if (c.tile == 128) {
+      matmul_kernel<DT, 128, 128, 2, 2, true><<<grid, dim3(256), 0, stream>>>(args);
     } else {
-      if (aligned) matmul_kernel<DT, 64, 64, 2, 2, true><<<grid, dim3(256), 0, stream>>>(args);
+      if (aligned) matmul_deep_kernel<DT, 64, 64, 2, 2><<<grid, dim3(256), 0, stream>>>(args);
       else matmul_kernel<DT, 64, 64, 2, 2, false><<<grid, dim3(256), 0, stream>>>(args);
     }
     OPTIMI_INT8_TRY(hipGetLastError());
     if (c.splits > 1) {
-      matmul_finish_kernel<DT><<<dim3((unsigned)((n + 1023) / 1024), (unsigned)(m < 65535 ? m : 65535)), dim3(256), 0, stream>>>(args);
+      const int64_t blocks = (m * n + 1023) / 1024;
+      matmul_finish_kernel<DT><<<dim3((unsigned)(blocks < 65536 ? blocks : 65536)), dim3(256), 0, stream>>>(args);
       OPTIMI_INT8_TRY(hipGetLastError());
     }
     return 0;
   });
 }
 
-// The workspace: partial sums of the split product, then those of the bias gradient.
 int64_t optimi_hip_int8_weight_grad_workspace(int64_t rows, int64_t outs, int64_t cols, int dtype, int with_bias) {
   if (!valid_dtype(dtype)) return OPTIMI_ERR_DTYPE;
   if (int rc = check_shape(rows, outs)) return rc;
   if (int rc = check_shape(rows, cols)) return rc;
   if (outs > kMostWidth || cols > kMostWidth) return OPTIMI_ERR_SIZE;
   if (outs == 0) return 0;
-  const Cut c = cols ? weight_grad_cut(rows, outs, cols, dtype) : Cut{1, 1, 1, 0};
-  return (c.splits > 1 ? c.splits * outs * cols * 4 : 0) + (with_bias ? column_sum_workspace(rows, outs) : 0);
+  const WeightGradPlan plan = weight_grad_plan(rows, outs, cols, dtype, with_bias != 0);
+  return plan.pad_bytes + plan.partial_bytes + plan.bias_bytes;
 }
 
 int optimi_hip_int8_weight_grad(const void* grad, const int8_t* values, const float* scales, int64_t rows, int64_t outs, int64_t cols, int dtype,
@@ -947,20 +1247,31 @@ int optimi_hip_int8_weight_grad(const void* grad, const int8_t* values, const fl
   if (int rc = check_shape(rows, cols)) return rc;
   if (outs > kMostWidth || cols > kMostWidth) return OPTIMI_ERR_SIZE;
   if (outs == 0) return 0;
-  if ((cols && !weight_grad) || (rows && (!grad || !scales || (cols && !values))) || (rows && bias_grad && !workspace)) return OPTIMI_ERR_NULL;
+  if ((cols && !weight_grad) || (rows && (!grad || !scales || (cols && !values)))) return OPTIMI_ERR_NULL;
   const int64_t size = elem_bytes(dtype);
-  if (!aligned_to(grad, size) || !aligned_to(scales, 4) || !aligned_to(weight_grad, size) || !aligned_to(bias_grad, size) || !aligned_to(workspace, 4))
+  if (!aligned_to(grad, size) || !aligned_to(scales, 4) || !aligned_to(weight_grad, size) || !aligned_to(bias_grad, size) || !aligned_to(workspace, 16))
     return OPTIMI_ERR_ALIGN;
+  const WeightGradPlan plan = weight_grad_plan(rows, outs, cols, dtype, bias_grad != nullptr);
+  if (plan.pad_bytes + plan.partial_bytes + plan.bias_bytes > 0 && !workspace) return OPTIMI_ERR_NULL;
   hipStream_t stream = (hipStream_t)stream_;
-  const Cut c = cols ? weight_grad_cut(rows, outs, cols, dtype) : Cut{1, 1, 1, 0};
-  if (c.tiles * c.splits > kMostTiles) return OPTIMI_ERR_SIZE;
-  if (c.splits > 1 && !workspace) return OPTIMI_ERR_NULL;
+  int8_t* work = (int8_t*)workspace;
   if (bias_grad) {
-    float* sums = (float*)workspace + (c.splits > 1 ? c.splits * outs * cols : 0);
-    if (int rc = column_sum(grad, rows, outs, dtype, bias_grad, sums, stream)) return rc;
+    if (int rc = column_sum(grad, rows, outs, dtype, bias_grad, work + plan.pad_bytes + plan.partial_bytes, stream)) return rc;
   }
   if (cols == 0) return 0;
-  const WeightGradArgs args{grad, values, scales, rows, outs, cols, weight_grad, (float*)workspace, c.splits, c.steps_per_split};
+  Cut c = plan.cut;
+  WeightGradArgs args{grad, outs, values, scales, rows, outs, cols, weight_grad, (float*)(work + plan.pad_bytes), c.splits, c.steps_per_split};
+  if (plan.pad) {
+    if (int rc = pad_rows(grad, rows, nullptr, 0, outs * 2, work, stream)) return rc;
+    args.grad = work;
+    args.stride = padded(outs * 2) / 2;
+  }
+  const bool direct = args.stride % 8 == 0 && aligned_to(args.grad, 16);
+  if (c.tile == 256 && !direct) {
+    c.tile = 128;
+    c.tiles = tiles_of(outs, cols, 128);
+  }
+  if (c.tiles * c.splits > kMostTiles) return OPTIMI_ERR_SIZE;
   return by_dtype(dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     const dim3 grid((unsigned)(c.tiles * c.splits));
@@ -969,14 +1280,9 @@ int optimi_hip_int8_weight_grad(const void* grad, const int8_t* values, const fl
     } else if constexpr (DT == OPTIMI_F32) {
       weight_grad_kernel<DT, 128, 128, 2, 2, 32, false><<<grid, dim3(256), 0, stream>>>(args);
     } else {
-      const bool direct = outs % 8 == 0 && aligned_to(grad, 16);
-      if (c.tile == 256) {
-        if (direct) weight_grad_wide_kernel<DT><<<grid, dim3(512), 0, stream>>>(args);
-        else weight_grad_kernel<DT, 256, 256, 2, 4, 64, false><<<grid, dim3(512), 0, stream>>>(args);
-      } else {
-        if (direct) weight_grad_kernel<DT, 128, 128, 2, 2, 64, true><<<grid, dim3(256), 0, stream>>>(args);
-        else weight_grad_kernel<DT, 128, 128, 2, 2, 64, false><<<grid, dim3(256), 0, stream>>>(args);
-      }
+      if (c.tile == 256) weight_grad_wide_kernel<DT><<<grid, dim3(512), 0, stream>>>(args);
+      else if (direct) weight_grad_kernel<DT, 128, 128, 2, 2, 64, true><<<grid, dim3(256), 0, stream>>>(args);
+      else weight_grad_kernel<DT, 128, 128, 2, 2, 64, false><<<grid, dim3(256), 0, stream>>>(args);
     }
     OPTIMI_INT8_TRY(hipGetLastError());
     if (c.splits > 1) {
