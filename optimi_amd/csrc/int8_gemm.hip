@@ -11,6 +11,9 @@ typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef short s16x8 __attribute__((ext_vector_type(8)));
 
+// The kernels' steps are written as lambdas over their sums and tiles; one that is called instead of inlined would send all
+// of them through memory.
+#define OPTIMI_INLINE __attribute__((always_inline))
 #define OPTIMI_LDS __attribute__((address_space(3)))
 #define OPTIMI_GLOBAL __attribute__((address_space(1)))
 
@@ -243,7 +246,7 @@ struct MatmulTile {
   template <bool LAST>
   __device__ __forceinline__ void multiply(const int8_t* ta, const int8_t* tb) {
     i32x4 fa[2][kM], fb[2][kN];
-    auto read = [&](int ks, i32x4(&ra)[kM], i32x4(&rb)[kN]) {
+    auto read = [&](int ks, i32x4(&ra)[kM], i32x4(&rb)[kN]) OPTIMI_INLINE {
 #pragma unroll
       for (int j = 0; j < kN; ++j) {
         rb[j] = TB::read(tb, wn + j * 32 + lane % 32, ks * 2 + lane / 32);
@@ -322,7 +325,7 @@ __global__ void __launch_bounds__(WM * WN * 64) matmul_kernel(MatmulArgs p) {
   const int rows_a = tile.rows_a(), rows_b = tile.rows_b();
   const uint32_t len = (uint32_t)p.k;
   const Buffer ra = buffer_of(tile.a(), rows_a * p.k), rb = buffer_of(tile.b(), rows_b * p.k);
-  auto fetch = [&](int step, auto which) {
+  auto fetch = [&](int step, auto which) OPTIMI_INLINE {
     if constexpr (ALIGNED) {
       TA::copy(ra, len, step * kStep, which.value ? a1 : a0);
       TB::copy(rb, len, step * kStep, which.value ? b1 : b0);
@@ -331,7 +334,7 @@ __global__ void __launch_bounds__(WM * WN * 64) matmul_kernel(MatmulArgs p) {
       TB::load(tile.b(), rows_b, len, step * kStep, vb);
     }
   };
-  auto fetch_last = [&](int step, auto which) {
+  auto fetch_last = [&](int step, auto which) OPTIMI_INLINE {
     if constexpr (ALIGNED) {
       fetch(step, which);
     } else {
@@ -339,7 +342,7 @@ __global__ void __launch_bounds__(WM * WN * 64) matmul_kernel(MatmulArgs p) {
       TB::load_last(tile.b(), rows_b, len, step * kStep, vb);
     }
   };
-  auto settle = [&](auto which) {
+  auto settle = [&](auto which) OPTIMI_INLINE {
     if constexpr (!ALIGNED) {
       TA::store(va, which.value ? a1 : a0);
       TB::store(vb, which.value ? b1 : b0);
@@ -347,8 +350,8 @@ __global__ void __launch_bounds__(WM * WN * 64) matmul_kernel(MatmulArgs p) {
     meet();
   };
   run_steps(tile.begin, tile.end, fetch, fetch_last, settle,
-            [&](auto which) { tile.template multiply<false>(which.value ? a1 : a0, which.value ? b1 : b0); },
-            [&](auto which) { tile.template multiply<true>(which.value ? a1 : a0, which.value ? b1 : b0); });
+            [&](auto which) OPTIMI_INLINE { tile.template multiply<false>(which.value ? a1 : a0, which.value ? b1 : b0); },
+            [&](auto which) OPTIMI_INLINE { tile.template multiply<true>(which.value ? a1 : a0, which.value ? b1 : b0); });
   // the second pair of tiles is free
   static_assert(M::kWaves / 2 * M::O::kBytes <= BM * kStep && M::kWaves / 2 * M::O::kBytes <= BN * kStep, "half of the waves' blocks fit either tile");
   tile.store((uint32_t*)((tile.wave < M::kWaves / 2 ? a1 : b1) + tile.wave % (M::kWaves / 2) * M::O::kBytes));
@@ -368,13 +371,13 @@ __global__ void __launch_bounds__(WM * WN * 64) matmul_deep_kernel(MatmulArgs p)
   const Buffer ra = buffer_of(tile.a(), tile.rows_a() * p.k), rb = buffer_of(tile.b(), tile.rows_b() * p.k);
   // Steps behind the end are fetched as well, so that the number of copies on their way is always the same; their
   // addresses lie outside of the buffers and nothing is read.
-  auto fetch = [&](int step, int8_t* a, int8_t* b) {
+  auto fetch = [&](int step, int8_t* a, int8_t* b) OPTIMI_INLINE {
     const uint32_t k0 = step < tile.end ? (uint32_t)step * kStep : 0x40000000u;
     TA::copy(ra, len, k0, a);
     TB::copy(rb, len, k0, b);
   };
   // This wave's copies but those of the two youngest steps have landed, then everybody's have; the step before is read.
-  auto meet_early = [&]() {
+  auto meet_early = [&]() OPTIMI_INLINE {
     constexpr int kYoung = 2 * (TA::kPieces + TB::kPieces);
     static_assert(kYoung == 8, "the count in the instruction below");
     asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory");
@@ -384,7 +387,7 @@ __global__ void __launch_bounds__(WM * WN * 64) matmul_deep_kernel(MatmulArgs p)
     fetch(begin, a0, b0);
     fetch(begin + 1, a1, b1);
     fetch(begin + 2, a2, b2);
-    auto one = [&](int at, int8_t* a, int8_t* b, int8_t* next_a, int8_t* next_b, auto last) {
+    auto one = [&](int at, int8_t* a, int8_t* b, int8_t* next_a, int8_t* next_b, auto last) OPTIMI_INLINE {
       meet_early();
       fetch(at + 3, next_a, next_b);
       __builtin_amdgcn_sched_barrier(0);
@@ -444,7 +447,7 @@ __global__ void __launch_bounds__(256) matvec_kernel(MatmulArgs p) {
   const int8_t* row[kRowsB];
 #pragma unroll
   for (int r = 0; r < kRowsB; ++r) row[r] = p.b + (n0 + r < p.n ? n0 + r : p.n - 1) * p.k;  // rows behind the last: the last again
-  auto some = [&](int64_t k, auto whole) {
+  auto some = [&](int64_t k, auto whole) OPTIMI_INLINE {
     u32x4 w[kRowsB], x[M];
 #pragma unroll
     for (int r = 0; r < kRowsB; ++r) w[r] = whole.value ? *(const u32x4_align1*)(row[r] + k) : load_bytes(row[r], k, p.k);
@@ -588,16 +591,22 @@ struct Product<OPTIMI_F32> : Product<OPTIMI_BF16> {
   static constexpr int kPieces = 3;
 };
 
-// The upper 8 bits of two fp32 numbers as two bf16 ones; what is left of them stays in x.  Three times over, the
-// pieces add up to the number exactly.  Numbers that are not finite leave nothing.
+// The upper 8 bits of two fp32 numbers as two bf16 ones; what is left of them stays in x and y.  Three times over, the
+// pieces add up to a finite number exactly.
 __device__ __forceinline__ uint32_t split_pair(float& x, float& y) {
   const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
-  const bool fx = abs_bits(x) < 0x7f800000u, fy = abs_bits(y) < 0x7f800000u;
-  x = fx ? x - __uint_as_float(a & 0xffff0000u) : 0.0f;
-  y = fy ? y - __uint_as_float(b & 0xffff0000u) : 0.0f;
-  // a NaN whose upper half would be an infinity's becomes a quiet one
-  const uint32_t ha = a | ((a & 0x7fffffffu) > 0x7f800000u ? 0x400000u : 0u), hb = b | ((b & 0x7fffffffu) > 0x7f800000u ? 0x400000u : 0u);
-  return __builtin_amdgcn_perm(hb, ha, 0x07060302u);
+  x -= __uint_as_float(a & 0xffff0000u);
+  y -= __uint_as_float(b & 0xffff0000u);
+  return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+// An infinity or a NaN is its own first piece (a NaN stays one without its lower bits) and leaves nothing.
+__device__ __forceinline__ uint32_t split_pair_special(float& x, float& y) {
+  uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+  x = abs_bits(x) < 0x7f800000u ? x - __uint_as_float(a & 0xffff0000u) : 0.0f;
+  y = abs_bits(y) < 0x7f800000u ? y - __uint_as_float(b & 0xffff0000u) : 0.0f;
+  a |= (a & 0x7fffffffu) > 0x7f800000u ? 0x400000u : 0u;
+  b |= (b & 0x7fffffffu) > 0x7f800000u ? 0x400000u : 0u;
+  return __builtin_amdgcn_perm(b, a, 0x07060302u);
 }
 
 // The sum runs over rows, and both operands lie in memory with their rows' columns side by side, so the matrix
@@ -610,192 +619,35 @@ struct HalfTile {
   static __device__ __forceinline__ int at(int row, int chunk) { return row * C + ((chunk ^ (row & (kChunks - 1) & 15)) * 16); }  // in elements
 };
 
-template <int DT, int BN, int BC, int WN, int WC, int STEP, bool DIRECT, bool NARROW = false>
-__global__ void __launch_bounds__(WN * WC * 64) weight_grad_kernel(WeightGradArgs p) {
-  using E = Elem<DT>;
-  using T = typename E::type;
-  using P = Product<DT>;
-  constexpr int kWaves = WN * WC, kThreads = kWaves * 64, kN = BN / WN / 16, kC = BC / WC / 16;
-  constexpr int kPieces = P::kPieces;
-  using TG = HalfTile<BN>;
-  using TQ = HalfTile<BC>;
-  __shared__ __attribute__((aligned(1024))) short g0[kPieces * STEP * BN], g1[kPieces * STEP * BN], q0[STEP * BC], q1[STEP * BC];
-  const int tn = (int)((p.outs + BN - 1) / BN), tc = (int)((p.cols + BC - 1) / BC);
-  const int split = blockIdx.x / (tn * tc);
-  const Tile tile = tile_of(blockIdx.x % (tn * tc), tn, tc);
-  const int64_t n0 = (int64_t)tile.row * BN, c0 = (int64_t)tile.col * BC;
-  const int wave = wave_id(), lane = threadIdx.x % 64;
-  const int wn = wave / WC * (BN / WN), wc = wave % WC * (BC / WC);
-  const int all = (int)((p.rows + STEP - 1) / STEP);
-  const int begin = split * p.steps_per_split, end = begin + p.steps_per_split < all ? begin + p.steps_per_split : all;
+// Rows 32 ks .. 32 ks + 31 of 16 columns from `offset` on, as the matrix instruction takes them (in an order of rows that is the same
+// for both operands).
+template <int C>
+__device__ __forceinline__ s16x8 read_column(const short* tile, int offset, int ks) {
+  typedef OPTIMI_LDS s16x4* Ptr;
+  const short* from = tile + offset + ks * 32 * C;
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)from);
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(from + 16 * C));
+  return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+}
 
-  f32x4 acc[kN][kC];
+// Four values as 16-bit numbers: bytes as unsigned numbers are 128 too large, (u - 128) s has one rounding, and none
+// under a power of two.
+template <int DT>
+__device__ __forceinline__ u32x2 widen(uint32_t word, float s) {
+  const uint32_t u = word ^ 0x80808080u;
+  const float minus = -128.0f * s;
+  float f[4];
 #pragma unroll
-  for (int i = 0; i < kN; ++i)
-#pragma unroll
-    for (int j = 0; j < kC; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+  for (int e = 0; e < 4; ++e) f[e] = fmaf((float)((u >> (8 * e)) & 0xffu), s, minus);
+  return u32x2{Product<DT>::pair(f[0], f[1]), Product<DT>::pair(f[2], f[3])};
+}
 
-  // per lane: kGrad pieces of 8 gradients, kQ pieces of 16 values
-  constexpr int kGrad = STEP * BN / 8 / kThreads, kQ = STEP * BC / 16 / kThreads;
-  static_assert(kGrad * 8 * kThreads == STEP * BN && kQ * 16 * kThreads == STEP * BC, "whole pieces per lane");
-  typename E::Raw vg[kGrad];
-  float sg[kGrad];
-  u32x4 vq[kQ];
-  float sq[kQ];
-  const int outs = (int)(p.outs - n0 < BN ? p.outs - n0 : BN), cols = (int)(p.cols - c0 < BC ? p.cols - c0 : BC);
-  auto copy = [&](int64_t m0, int rows, short* g) {  // LDS place -> row, place in row; the source follows the swizzle
-    const Buffer from = buffer_of((const T*)p.grad + m0 * p.stride + n0, ((int64_t)(rows - 1) * p.stride + outs) * 2);
-#pragma unroll
-    for (int i = 0; i < kGrad; ++i) {
-      const int place = i * kThreads + threadIdx.x;
-      const int row = place / (BN / 8), in = place % (BN / 8);
-      const int n = TG::at(row, in / 2) - row * BN + in % 2 * 8;
-      copy16_to_lds(from, ((uint32_t)row * (uint32_t)p.stride + n) * 2, g + (i * kThreads + wave * 64) * 8);
-    }
-  };
-  // A full step's loads.  Columns behind the matrix are read from its first ones and never used; a piece that begins inside
-  // may run into the next row, of which there is one.
-  auto fetch = [&](int step, auto which) {
-    const int64_t m0 = (int64_t)step * STEP;
-    const T* grad = (const T*)p.grad + m0 * p.outs + n0;
-    const int8_t* values = p.values + m0 * p.cols + c0;
-    const float* scales = p.scales + m0;
-    if constexpr (DIRECT) {
-      copy(m0, STEP, which.value ? g1 : g0);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kGrad; ++i) {
-        const int place = i * kThreads + threadIdx.x;
-        const int row = place / (BN / 8), n = place % (BN / 8) * 8;
-        vg[i] = E::load(grad + ((uint32_t)row * (uint32_t)p.outs + (n < outs ? n : 0)));
-        if (kPieces > 1) sg[i] = scales[row];
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kQ; ++i) {
-      const int place = i * kThreads + threadIdx.x;
-      const int row = place / (BC / 16), c = place % (BC / 16) * 16;
-      vq[i] = *(const u32x4_align1*)(values + ((uint32_t)row * (uint32_t)p.cols + (c < cols ? c : 0)));
-      sq[i] = kPieces > 1 ? 1.0f : scales[row];
-    }
-  };
-  // The last step's, or any step's of a matrix that is narrower than a piece.
-  auto fetch_last = [&](int step, auto which) {
-    const int64_t m0 = (int64_t)step * STEP;
-    const T* grad = (const T*)p.grad + m0 * p.outs + n0;
-    const int8_t* values = p.values + m0 * p.cols + c0;
-    const float* scales = p.scales + m0;
-    const int rows = (int)(p.rows - m0 < STEP ? p.rows - m0 : STEP);
-    if constexpr (DIRECT) {
-      copy(m0, rows, which.value ? g1 : g0);
-    } else {
-#pragma unroll
-      for (int i = 0; i < kGrad; ++i) {
-        const int place = i * kThreads + threadIdx.x;
-        const int row = place / (BN / 8), n = place % (BN / 8) * 8;
-        const bool in = row < rows && n < outs;
-        vg[i] = in ? load_some<DT>(grad + (uint32_t)row * (uint32_t)p.outs + n, outs - n) : E::zero();
-        if (kPieces > 1) sg[i] = in ? scales[row] : 0.0f;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kQ; ++i) {
-      const int place = i * kThreads + threadIdx.x;
-      const int row = place / (BC / 16), c = place % (BC / 16) * 16;
-      const bool in = row < rows && c < cols;
-      vq[i] = in ? load_bytes(values + (uint32_t)row * (uint32_t)p.cols, c, cols) : u32x4{0, 0, 0, 0};
-      sq[i] = kPieces > 1 ? 1.0f : in ? scales[row] : 0.0f;
-    }
-  };
-  auto settle = [&](auto which) {
-    short *g = which.value ? g1 : g0, *q = which.value ? q1 : q0;
-    if constexpr (!DIRECT) {
-#pragma unroll
-      for (int i = 0; i < kGrad; ++i) {
-        const int place = i * kThreads + threadIdx.x;
-        const int row = place / (BN / 8), in = place % (BN / 8);
-        short* to = g + TG::at(row, in / 2) + in % 2 * 8;
-        if constexpr (kPieces == 1) {
-          *(u32x4*)to = vg[i].a;
-        } else {
-          float f[8];
-          E::unpack(vg[i], f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] *= sg[i];
-#pragma unroll
-          for (int z = 0; z < kPieces; ++z) {
-            u32x4 v;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = split_pair(f[2 * e], f[2 * e + 1]);
-            *(u32x4*)(to + z * STEP * BN) = v;
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kQ; ++i) {
-      const int place = i * kThreads + threadIdx.x;
-      short* to = q + TQ::at(place / (BC / 16), place % (BC / 16));
-      const float s = sq[i], minus = -128.0f * s;
-      u32x4 v[2];
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        // bytes as unsigned numbers, 128 too large: (u - 128) s with one rounding
-        const uint32_t u = vq[i][w] ^ 0x80808080u;
-        float f[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = fmaf((float)((u >> (8 * e)) & 0xffu), s, minus);
-        v[w / 2][w % 2 * 2] = P::pair(f[0], f[1]);
-        v[w / 2][w % 2 * 2 + 1] = P::pair(f[2], f[3]);
-      }
-      *(u32x4*)to = v[0];
-      *(u32x4*)(to + 8) = v[1];
-    }
-    meet();
-  };
-  // rows 32 ks .. 32 ks + 31 of 16 columns, as the matrix instruction takes them (in an order of rows that is the same for both operands)
-  auto column = [&](const short* t, int pitch, int offset, int ks) {
-    typedef OPTIMI_LDS s16x4* Ptr;
-    const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(t + offset + ks * 32 * pitch));
-    const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(t + offset + (ks * 32 + 16) * pitch));
-    return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-  };
-  // `left`: rows of the sum that are left.  The values behind them are zeros, but a copied gradient tile holds
-  // whatever was in LDS there, infinities maybe.
-  const int left = end == all ? (int)(p.rows - (int64_t)(all - 1) * STEP) : STEP;
-  auto multiply_some = [&](const short* g, const short* q, auto last) {
-#pragma unroll
-    for (int ks = 0; ks < STEP / 32; ++ks) {
-      s16x8 fq[kC], keep;
-      if (last.value) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) keep[e] = ks * 32 + e / 4 * 16 + lane / 16 * 4 + e % 4 < left ? -1 : 0;
-      }
-#pragma unroll
-      for (int j = 0; j < kC; ++j) fq[j] = column(q, BC, TQ::at(lane / 4, wc / 16 + j) + lane % 4 * 4, ks);
-#pragma unroll
-      for (int z = kPieces - 1; z >= 0; --z)
-#pragma unroll
-        for (int i = 0; i < kN; ++i) {
-          s16x8 fg = column(g + z * STEP * BN, BN, TG::at(lane / 4, wn / 16 + i) + lane % 4 * 4, ks);
-          if (last.value) fg &= keep;
-#pragma unroll
-          for (int j = 0; j < kC; ++j) acc[i][j] = P::mfma(fq[j], fg, acc[i][j]);
-        }
-    }
-  };
-
-  auto fetch_any = [&](int step, auto which) {
-    if constexpr (NARROW) fetch_last(step, which);
-    else fetch(step, which);
-  };
-  run_steps(begin, end, fetch_any, fetch_last, settle, [&](auto which) { multiply_some(which.value ? g1 : g0, which.value ? q1 : q0, std::false_type{}); },
-            [&](auto which) { multiply_some(which.value ? g1 : g0, which.value ? q1 : q0, std::bool_constant<DIRECT>{}); });
-
-  using O = OutBlock<16, BC / WC>;
-  static_assert(kWaves / 2 * O::kBytes <= STEP * BC * 2 && kWaves / 2 * O::kBytes <= STEP * BN * 2, "half of the waves' blocks fit either tile");
-  uint32_t* block = (uint32_t*)((char*)(wave < kWaves / 2 ? g1 : q1) + wave % (kWaves / 2) * O::kBytes);
-  const int64_t c = c0 + wc + O::col();
+// A wave's 16 kN x 16 kC sums, 16 rows at a time through LDS.
+template <int DT, class O, int kN, int kC>
+__device__ __forceinline__ void store_sums(const WeightGradArgs& p, const f32x4 (&acc)[kN][kC], uint32_t* block, int split, int64_t n0, int64_t c0) {
+  using T = typename Elem<DT>::type;
+  const int lane = threadIdx.x % 64;
+  const int64_t c = c0 + O::col();
   const int64_t some = p.cols - c;
 #pragma unroll
   for (int i = 0; i < kN; ++i) {
@@ -804,7 +656,7 @@ __global__ void __launch_bounds__(WN * WC * 64) weight_grad_kernel(WeightGradArg
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int t = 0; t < O::kTurns; ++t) {
-      const int64_t n = n0 + wn + i * 16 + O::row(t);
+      const int64_t n = n0 + i * 16 + O::row(t);
       uint32_t v[8];
       O::get(block, O::row(t), v);
       const float(&f)[8] = reinterpret_cast<const float(&)[8]>(v);
@@ -815,6 +667,212 @@ __global__ void __launch_bounds__(WN * WC * 64) weight_grad_kernel(WeightGradArg
     }
     __builtin_amdgcn_wave_barrier();
   }
+}
+
+// 128 x 128 tiles, 64 rows a step, two pairs of tiles in LDS, eight wavefronts with 64 x 32 sums each.  Both operands go through
+// registers, from any address: they are loaded two steps ahead, turned into what the matrix instruction takes while
+// the step before theirs is multiplied, and written to LDS.  fp32 gradients are multiplied by their row's scale and split into
+// three bf16 pieces, so that their products are exact and cost three times as many instructions; the values are
+// whole numbers there.  NARROW: rows are shorter than a piece of a load, every load looks at the borders.
+template <int DT, bool NARROW>
+__global__ void __launch_bounds__(512) weight_grad_kernel(WeightGradArgs p) {
+  using E = Elem<DT>;
+  using T = typename E::type;
+  using P = Product<DT>;
+  constexpr int kTile = 128, kRows = 64, kWaves = 8, kN = 4, kC = 2, kGrad = 2, kPieces = P::kPieces;
+  constexpr int kPlane = kRows * kTile;
+  using H = HalfTile<kTile>;
+  __shared__ __attribute__((aligned(1024))) short g0[kPieces * kPlane], g1[kPieces * kPlane], q0[kPlane], q1[kPlane];
+  const int tn = (int)((p.outs + kTile - 1) / kTile), tc = (int)((p.cols + kTile - 1) / kTile);
+  const int split = blockIdx.x / (tn * tc);
+  const Tile tile = tile_of(blockIdx.x % (tn * tc), tn, tc);
+  const int64_t n0 = (int64_t)tile.row * kTile, c0 = (int64_t)tile.col * kTile;
+  const int wave = wave_id(), lane = threadIdx.x % 64;
+  const int wn = wave / 4 * 64, wc = wave % 4 * 32;
+  const int all = (int)((p.rows + kRows - 1) / kRows);
+  const int begin = split * p.steps_per_split, end = begin + p.steps_per_split < all ? begin + p.steps_per_split : all;
+
+  f32x4 acc[kN][kC];
+#pragma unroll
+  for (int i = 0; i < kN; ++i)
+#pragma unroll
+    for (int j = 0; j < kC; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+
+  // a lane's part of a step: eight gradients of each of two rows, sixteen values of one
+  struct Part {
+    typename E::Raw g[kGrad];
+    float sg[kGrad];
+    u32x4 q;
+    float sq;
+  };
+  Part part[2];
+  const int outs = (int)(p.outs - n0 < kTile ? p.outs - n0 : kTile), cols = (int)(p.cols - c0 < kTile ? p.cols - c0 : kTile);
+  const int g_row = threadIdx.x / 16, g_col = threadIdx.x % 16 * 8, q_row = threadIdx.x / 8, q_col = threadIdx.x % 8 * 16;
+  // Columns behind the matrix are read from its first ones and never used; a piece that begins inside may run into the next
+  // row, of which there is one in all steps but the last.  The last step's loads look at the borders, and bring zeros from behind them.
+  auto load = [&](int step, Part& v, auto last) OPTIMI_INLINE {
+    const int64_t m0 = (int64_t)step * kRows;
+    const T* grad = (const T*)p.grad + m0 * p.stride + n0;
+    const int8_t* values = p.values + m0 * p.cols + c0;
+    const float* scales = p.scales + m0;
+    if constexpr (!NARROW && !last.value) {
+#pragma unroll
+      for (int i = 0; i < kGrad; ++i) {
+        v.g[i] = E::load(grad + ((uint32_t)(g_row + i * 32) * (uint32_t)p.stride + (g_col < outs ? g_col : 0)));
+        if (kPieces > 1) v.sg[i] = scales[g_row + i * 32];
+      }
+      v.q = *(const u32x4_align1*)(values + ((uint32_t)q_row * (uint32_t)p.cols + (q_col < cols ? q_col : 0)));
+      if (kPieces == 1) v.sq = scales[q_row];
+    } else {
+      const int rows = (int)(p.rows - m0 < kRows ? p.rows - m0 : kRows);
+#pragma unroll
+      for (int i = 0; i < kGrad; ++i) {
+        const bool in = g_row + i * 32 < rows && g_col < outs;
+        v.g[i] = E::zero();
+        if (in) v.g[i] = load_some<DT>(grad + ((uint32_t)(g_row + i * 32) * (uint32_t)p.stride + g_col), outs - g_col);
+        if (kPieces > 1) v.sg[i] = in ? scales[g_row + i * 32] : 0.0f;
+      }
+      const bool in = q_row < rows && q_col < cols;
+      v.q = in ? load_bytes(values + (uint32_t)q_row * (uint32_t)p.cols, q_col, cols) : u32x4{0, 0, 0, 0};
+      if (kPieces == 1) v.sq = in ? scales[q_row] : 0.0f;
+    }
+  };
+  // Turning a part into 16-bit tiles, in as many pieces of work as a step has groups of products, between which they go.  Of
+  // an fp32 row's eight numbers two at a time give their next bf16 piece, and after the fourth pair that piece is written.
+  constexpr int kGroups = 2 * kPieces * kN;  // groups of kC products in a step
+  struct Turn {
+    float f[8];
+    u32x4 w, q[2];
+    uint32_t most;
+  };
+  auto grad_place = [&](int i, short* g) OPTIMI_INLINE { return g + H::at(g_row + i * 32, g_col / 16) + g_col % 16; };
+  auto turn_values = [&](int word, const Part& v, Turn& t, short* q) OPTIMI_INLINE {
+    const u32x2 two = widen<DT>(v.q[word], kPieces > 1 ? 1.0f : v.sq);
+    t.q[word / 2][word % 2 * 2] = two[0];
+    t.q[word / 2][word % 2 * 2 + 1] = two[1];
+    if (word % 2) *(u32x4*)(q + H::at(q_row, q_col / 16) + word / 2 * 8) = t.q[word / 2];
+  };
+  auto turn = [&](int at, const Part& v, Turn& t, short* g, short* q) OPTIMI_INLINE {
+    if constexpr (kPieces == 1) {
+      if (at < kGrad) *(u32x4*)grad_place(at, g) = v.g[at].a;
+      if (at >= kGroups - 4) turn_values(at - (kGroups - 4), v, t, q);
+    } else {
+      const int i = at / 12, z = at % 12 / 4, e = at % 4;  // the row, the piece, the pair
+      if (at % 12 == 0) {
+        E::unpack(v.g[i], t.f);
+        if (i == 0) t.most = 0;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          t.f[k] *= v.sg[i];
+          t.most = MaxOp::join(t.most, abs_bits(t.f[k]));
+        }
+      }
+      t.w[e] = split_pair(t.f[2 * e], t.f[2 * e + 1]);
+      if (e == 3) *(u32x4*)(grad_place(i, g) + z * kPlane) = t.w;
+      if (at % 6 == 5) turn_values(at / 6, v, t, q);
+    }
+  };
+  // The rows that hold an infinity or a NaN again: such a number leaves nothing to its further pieces.
+  auto turn_special = [&](const Part& v, const Turn& t, short* g) OPTIMI_INLINE {
+    if constexpr (kPieces > 1) {
+      if (t.most < 0x7f800000u) return;
+#pragma unroll
+      for (int i = 0; i < kGrad; ++i) {
+        float f[8];
+        E::unpack(v.g[i], f);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) f[k] *= v.sg[i];
+#pragma unroll
+        for (int z = 0; z < kPieces; ++z) {
+          u32x4 w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = split_pair_special(f[2 * e], f[2 * e + 1]);
+          *(u32x4*)(grad_place(i, g) + z * kPlane) = w;
+        }
+      }
+    }
+  };
+  auto multiply = [&](const short* g, const short* q, auto more, const Part& v, short* next_g, short* next_q) OPTIMI_INLINE {
+    s16x8 fq[2][kC], fg[3];
+    Turn t;
+    auto read_g = [&](int at) OPTIMI_INLINE {  // the smallest pieces first
+      const int ks = at / (kGroups / 2), z = kPieces - 1 - at % (kGroups / 2) / kN, i = at % kN;
+      return read_column<kTile>(g + z * kPlane, H::at(lane / 4, wn / 16 + i) + lane % 4 * 4, ks);
+    };
+    auto read_q = [&](int ks) OPTIMI_INLINE {
+#pragma unroll
+      for (int j = 0; j < kC; ++j) fq[ks][j] = read_column<kTile>(q, H::at(lane / 4, wc / 16 + j) + lane % 4 * 4, ks);
+    };
+    read_q(0);
+    fg[0] = read_g(0);
+    fg[1] = read_g(1);
+#pragma unroll
+    for (int at = 0; at < kGroups; ++at) {
+      if (at + 2 < kGroups) fg[(at + 2) % 3] = read_g(at + 2);
+      if (at == kGroups / 2 - 2) read_q(1);
+#pragma unroll
+      for (int j = 0; j < kC; ++j) acc[at % kN][j] = P::mfma(fq[at / (kGroups / 2)][j], fg[at % 3], acc[at % kN][j]);
+      if (more.value) turn(at, v, t, next_g, next_q);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (more.value) turn_special(v, t, next_g);
+  };
+  // One step, with the loads of the next but one: an ordinary step's, the last one's, or none.  They are not told apart inside
+  // the loop: a branch around loads makes the compiler wait for all of them in front of the next ones.
+  const std::false_type ordinary;
+  const std::true_type last;
+  auto step_on = [&](int step, auto which, auto loads) OPTIMI_INLINE {
+    constexpr int W = decltype(which)::value;
+    loads(step + 2, part[W]);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(W ? g1 : g0, W ? q1 : q0, std::true_type{}, part[1 - W], W ? g0 : g1, W ? q0 : q1);
+    __syncthreads();
+  };
+  auto load_next = [&](int step, Part& v) OPTIMI_INLINE { load(step, v, ordinary); };
+  auto load_last = [&](int step, Part& v) OPTIMI_INLINE { load(step, v, last); };
+  auto load_none = [&](int, Part&) OPTIMI_INLINE {};
+  auto start = [&](auto which) OPTIMI_INLINE {
+    constexpr int W = decltype(which)::value;
+    Turn t;
+#pragma unroll
+    for (int at = 0; at < kGroups; ++at) turn(at, part[W], t, W ? g1 : g0, W ? q1 : q0);
+    turn_special(part[W], t, W ? g1 : g0);
+    __syncthreads();
+  };
+  const Pair<0> p0;
+  const Pair<1> p1;
+  const int n = end - begin;  // the last step works on the first pair of tiles
+  if (n == 1) {
+    load(begin, part[0], last);
+    start(p0);
+  } else if (n == 2) {
+    load(begin, part[1], ordinary);
+    load(begin + 1, part[0], last);
+    start(p1);
+  } else if (n > 2) {
+    int step = begin;
+    if (n % 2) {
+      load(step, part[0], ordinary);
+      load(step + 1, part[1], ordinary);
+      start(p0);
+    } else {
+      load(step, part[1], ordinary);
+      load(step + 1, part[0], ordinary);
+      start(p1);
+      step_on(step++, p1, load_next);
+    }
+    for (; step + 3 < end; step += 2) {
+      step_on(step, p0, load_next);
+      step_on(step + 1, p1, load_next);
+    }
+    step_on(step++, p0, load_last);
+  }
+  if (n > 1) step_on(end - 2, p1, load_none);
+  if (n > 0) multiply(g0, q0, std::false_type{}, part[0], g1, q1);
+
+  using O = OutBlock<16, 32>;
+  static_assert(kWaves / 2 * O::kBytes <= kPlane * 2, "half of the waves' blocks fit a tile");
+  store_sums<DT, O, kN, kC>(p, acc, (uint32_t*)((char*)(wave < 4 ? g1 : q1) + wave % 4 * O::kBytes), split, n0 + wn, c0 + wc);
 }
 
 // The same for large 16-bit products, where all that counts is that the matrix instructions never wait: 256 x 256 tiles, 64
@@ -847,7 +905,7 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
   // Gradients: a wave's copy fills two rows of LDS; the sources follow the swizzle.  Columns behind the matrix come from the
   // next row (or not at all, behind the last) and end in sums that are not stored.
   const int width = (int)(p.stride - n0 < kTile ? p.stride - n0 : kTile);
-  auto copy = [&](int step, short* g) {
+  auto copy = [&](int step, short* g) OPTIMI_INLINE {
     const int64_t m0 = (int64_t)step * kRows;
     const int rows = (int)(p.rows - m0 < kRows ? p.rows - m0 : kRows);
     const Buffer from = buffer_of((const T*)p.grad + m0 * p.stride + n0, ((int64_t)(rows - 1) * p.stride + width) * 2);
@@ -867,7 +925,7 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
   const uint32_t col = (uint32_t)c0 + (c0 + at_col * 16 < p.cols ? at_col * 16 : 0);
   u32x4 vq[2][kPieces];
   float sq[2][kPieces];
-  auto place_of = [&](int step, int i, int64_t& start, uint32_t& limit) {
+  auto place_of = [&](int step, int i, int64_t& start, uint32_t& limit) OPTIMI_INLINE {
     const int64_t m0 = (int64_t)step * kRows, first = m0 * p.cols;
     start = first < total - 16 ? first : total - 16;
     const int64_t left = total - 16 - start;
@@ -875,7 +933,7 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
     const int rows = (int)(p.rows - m0 < kRows ? p.rows - m0 : kRows), row = at_row + i * 32;
     return (uint32_t)(row < rows ? row : rows - 1) * (uint32_t)p.cols + col + (uint32_t)(first - start);
   };
-  auto load = [&](int step, u32x4 (&v)[kPieces], float (&s)[kPieces]) {
+  auto load = [&](int step, u32x4 (&v)[kPieces], float (&s)[kPieces]) OPTIMI_INLINE {
     const int64_t m0 = (int64_t)step * kRows;
     const int rows = (int)(p.rows - m0 < kRows ? p.rows - m0 : kRows);
 #pragma unroll
@@ -888,7 +946,7 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
       s[i] = p.scales[m0 + (row < rows ? row : rows - 1)];
     }
   };
-  auto shift = [&](int step, u32x4 (&v)[kPieces], float (&s)[kPieces]) {  // the very last step only
+  auto shift = [&](int step, u32x4 (&v)[kPieces], float (&s)[kPieces]) OPTIMI_INLINE {  // the very last step only
     const int rows = (int)(p.rows - (int64_t)step * kRows);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
@@ -907,19 +965,9 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
       if (at_row + i * 32 >= rows) s[i] = 0.0f;
     }
   };
-  // Four values as 16-bit numbers: bytes as unsigned numbers are 128 too large, (u - 128) s has one rounding, and none
-  // under a power of two.
-  auto convert = [&](uint32_t word, float s) {
-    const uint32_t u = word ^ 0x80808080u;
-    const float minus = -128.0f * s;
-    float f[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = fmaf((float)((u >> (8 * e)) & 0xffu), s, minus);
-    return u32x2{P::pair(f[0], f[1]), P::pair(f[2], f[3])};
-  };
-  auto write_half = [&](int half, const u32x4 (&v)[kPieces], const float (&s)[kPieces], short* q) {  // eight values of piece half / 2
+  auto write_half = [&](int half, const u32x4 (&v)[kPieces], const float (&s)[kPieces], short* q) OPTIMI_INLINE {  // eight values of piece half / 2
     const int i = half / 2;
-    const u32x2 a = convert(v[i][half % 2 * 2], s[i]), b = convert(v[i][half % 2 * 2 + 1], s[i]);
+    const u32x2 a = widen<DT>(v[i][half % 2 * 2], s[i]), b = widen<DT>(v[i][half % 2 * 2 + 1], s[i]);
     *(u32x4*)(q + H::at(at_row + i * 32, at_col) + half % 2 * 8) = u32x4{a[0], a[1], b[0], b[1]};
   };
 
@@ -927,13 +975,13 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
   // exclusive or away from its first.  The addresses are formed anew for every step: kept over the loop, they would take more
   // registers than there are.
   typedef OPTIMI_LDS s16x4* Ptr;
-  auto column = [&](const short* t, int first, int i, int ks) {
+  auto column = [&](const short* t, int first, int i, int ks) OPTIMI_INLINE {
     const char* from = (const char*)t + (first ^ (i * 32)) + ks * 32 * kTile * 2;
     const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)from);
     const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(from + 16 * kTile * 2));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
   };
-  auto anew = [](int v) {
+  auto anew = [](int v) OPTIMI_INLINE {
     asm volatile("" : "+v"(v));
     return v & 0x7fff;
   };
@@ -941,10 +989,10 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
   const int left = end == all ? (int)(p.rows - (int64_t)(all - 1) * kRows) : kRows;
   // One step's products in sixteen groups; a group's operands are read two groups earlier, and four of the groups are followed
   // by a quarter of the next step's conversion.
-  auto multiply = [&](const short* g, const short* q, auto last, const u32x4 (&v)[kPieces], const float (&s)[kPieces], short* next) {
+  auto multiply = [&](const short* g, const short* q, auto last, const u32x4 (&v)[kPieces], const float (&s)[kPieces], short* next) OPTIMI_INLINE {
     const int at_g = anew(first_g), at_q = anew(first_q);
     s16x8 fq[2][kC], fg[3];
-    auto keep = [&](s16x8 f, int ks) {  // copied gradients of rows behind the last are whatever was in LDS, infinities maybe
+    auto keep = [&](s16x8 f, int ks) OPTIMI_INLINE {  // copied gradients of rows behind the last are whatever was in LDS, infinities maybe
       if (!last.value) return f;
       s16x8 mask;
 #pragma unroll
@@ -970,7 +1018,7 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  auto step_on = [&](int step, auto which) {
+  auto step_on = [&](int step, auto which) OPTIMI_INLINE {
     constexpr int W = decltype(which)::value;
     copy(step + 1, W ? g0 : g1);
     if (step + 2 < end) load(step + 2, vq[W], sq[W]);
@@ -979,7 +1027,7 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
     multiply(W ? g1 : g0, W ? q1 : q0, std::false_type{}, vq[1 - W], sq[1 - W], W ? q0 : q1);
     meet();
   };
-  auto start = [&](int step, auto which) {
+  auto start = [&](int step, auto which) OPTIMI_INLINE {
     constexpr int W = decltype(which)::value;
     copy(step, W ? g1 : g0);
     load(step, vq[W], sq[W]);
@@ -1007,42 +1055,34 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
   }
 
   using O = OutBlock<16, 64>;
-  uint32_t* block = (uint32_t*)((char*)(wave < 4 ? g1 : q1) + wave % 4 * O::kBytes);
-  const int64_t c = c0 + wc + O::col();
-  const int64_t some = p.cols - c;
-#pragma unroll
-  for (int i = 0; i < kN; ++i) {
-#pragma unroll
-    for (int j = 0; j < kC; ++j) O::put(block, lane % 16, j * 4 + lane / 16, __builtin_bit_cast(u32x4, acc[i][j]));
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int t = 0; t < O::kTurns; ++t) {
-      const int64_t n = n0 + wn + i * 16 + O::row(t);
-      uint32_t v[8];
-      O::get(block, O::row(t), v);
-      const float(&f)[8] = reinterpret_cast<const float(&)[8]>(v);
-      if (n < p.outs && some > 0) {
-        if (p.splits > 1) store_some<OPTIMI_F32>(p.partial + ((int64_t)split * p.outs + n) * p.cols + c, f, some);
-        else store_some<DT>((T*)p.out + n * p.cols + c, f, some);
-      }
-    }
-    __builtin_amdgcn_wave_barrier();
-  }
+  store_sums<DT, O, kN, kC>(p, acc, (uint32_t*)((char*)(wave < 4 ? g1 : q1) + wave % 4 * O::kBytes), split, n0 + wn, c0 + wc);
 }
 
-// Adds the splits' sums, always in the same order.
+// Adds the splits' sums, four neighbours a lane, always in the same order.
 template <int DT>
 __global__ void __launch_bounds__(256) weight_grad_finish_kernel(WeightGradArgs p) {
   using E = Elem<DT>;
+  typedef f32x4 f32x4_align4 __attribute__((aligned(4)));
   const int64_t n = p.outs * p.cols;
-  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; i < n; i += (int64_t)gridDim.x * 1024) {
+  for (int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; at < n; at += (int64_t)gridDim.x * 1024) {
+    const int some = (int)(n - at < 4 ? n - at : 4);
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (some == 4) {
+#pragma unroll 8
+      for (int s = 0; s < p.splits; ++s) {
+        const f32x4 v = *(const f32x4_align4*)(p.partial + s * n + at);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (i + e >= n) break;
-      float sum = 0.0f;
-      for (int s = 0; s < p.splits; ++s) sum += p.partial[s * n + i + e];
-      ((typename E::type*)p.out)[i + e] = E::put(sum);
+        for (int e = 0; e < 4; ++e) sum[e] += v[e];
+      }
+    } else {
+      for (int s = 0; s < p.splits; ++s)
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          if (e < some) sum[e] += p.partial[s * n + at + e];
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < some) ((typename E::type*)p.out)[at + e] = E::put(sum[e]);
   }
 }
 
@@ -1073,6 +1113,12 @@ struct Cut {
 constexpr int kCus = 256;
 inline int64_t tiles_of(int64_t rows, int64_t cols, int tile) { return ((rows + tile - 1) / tile) * ((cols + tile - 1) / tile); }
 
+// Which tile: the one whose steps, for all of its tiles, take the least time.  Measured in microseconds per step of 128 bytes on
+// the whole machine, int8 operands that come from the caches: 256 x 256 tiles 1.55 where they leave half of the 256 CUs empty,
+// 2.05 per round of 256; 128 x 128 tiles 0.68, 0.82 up to one per CU, 1.2 per round of two per CU; 64 x 64 tiles 0.25 up to
+// one per CU, then 0.22 for each further one.  (2048 x 4096 x 4096: 52 us in tiles of 256, 41 in tiles of 128, 60 in
+// tiles of 64; 4096 x 4096 x 4096: 66, 77, 112; 512 x 4096 x 4096: 47, 24, 18.)  Few tiles with a long sum are split, one part
+// per idle CU, eight steps at least each: 100 x 100 x 16384 takes 23 us whole and 9.2 us in 16 parts.
 Cut matmul_cut(int64_t m, int64_t n, int64_t k) {
   const int64_t steps = (k + kStep - 1) / kStep;
   const int64_t t256 = tiles_of(m, n, 256), t128 = tiles_of(m, n, 128), t64 = tiles_of(m, n, 64);
@@ -1087,11 +1133,18 @@ Cut matmul_cut(int64_t m, int64_t n, int64_t k) {
   c.split(steps, parts < 16 ? parts : 16);
   return c;
 }
+// The same for weight gradients, in microseconds per step of 64 rows: 2.2 per round of 256 wide tiles; 0.8 for up to 256 tiles
+// of 128 x 128, 1.45 per round of two per CU.  (1024 x 4096 x 4096: 43 us in wide tiles, 61 in the others; 2048 x 2048 x 2048:
+// 66, 28.)  Four steps at least to a part: 4096 x 512 x 512 takes 44 us whole, 17 us in eight parts.
 Cut weight_grad_cut(int64_t rows, int64_t outs, int64_t cols, int dtype) {
   const bool narrow = outs < 8 || cols < 16;
-  const int64_t steps = dtype == OPTIMI_F32 || narrow ? (rows + 31) / 32 : (rows + 63) / 64;
+  const int64_t steps = (rows + 63) / 64;
   Cut c;
-  c.tile = dtype != OPTIMI_F32 && !narrow && tiles_of(outs, cols, 256) >= kCus / 2 && rows * cols >= 16 ? 256 : 128;
+  const int64_t t256 = tiles_of(outs, cols, 256), t128 = tiles_of(outs, cols, 128);
+  const double c256 = 2.2 * (double)((t256 + kCus - 1) / kCus);
+  const double c128 = t128 <= kCus ? 0.8 : 1.45 * (double)((t128 + 2 * kCus - 1) / (2 * kCus));
+  const bool wide = dtype != OPTIMI_F32 && !narrow && rows * cols >= 16;
+  c.tile = wide && t256 >= kCus / 2 && c256 <= c128 ? 256 : 128;
   c.tiles = tiles_of(outs, cols, c.tile);
   int64_t parts = 1;
   if (c.tiles < kCus) parts = kCus / c.tiles < steps / 4 ? kCus / c.tiles : steps / 4;
@@ -1275,14 +1328,12 @@ int optimi_hip_int8_weight_grad(const void* grad, const int8_t* values, const fl
   return by_dtype(dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     const dim3 grid((unsigned)(c.tiles * c.splits));
-    if (outs < 8 || cols < 16) {  // too narrow for whole pieces: every step looks at the borders
-      weight_grad_kernel<DT, 128, 128, 2, 2, 32, false, true><<<grid, dim3(256), 0, stream>>>(args);
-    } else if constexpr (DT == OPTIMI_F32) {
-      weight_grad_kernel<DT, 128, 128, 2, 2, 32, false><<<grid, dim3(256), 0, stream>>>(args);
+    if (c.tile == 256) {
+      if constexpr (DT != OPTIMI_F32) weight_grad_wide_kernel<DT><<<grid, dim3(512), 0, stream>>>(args);
+    } else if (outs < 8 || cols < 16) {  // too narrow for whole pieces
+      weight_grad_kernel<DT, true><<<grid, dim3(512), 0, stream>>>(args);
     } else {
-      if (c.tile == 256) weight_grad_wide_kernel<DT><<<grid, dim3(512), 0, stream>>>(args);
-      else if (direct) weight_grad_kernel<DT, 128, 128, 2, 2, 64, true><<<grid, dim3(256), 0, stream>>>(args);
-      else weight_grad_kernel<DT, 128, 128, 2, 2, 64, false><<<grid, dim3(256), 0, stream>>>(args);
+      weight_grad_kernel<DT, false><<<grid, dim3(512), 0, stream>>>(args);
     }
     OPTIMI_INT8_TRY(hipGetLastError());
     if (c.splits > 1) {
