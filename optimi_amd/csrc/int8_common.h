@@ -124,13 +124,16 @@ struct Elem<OPTIMI_F16> {
   }
 };
 
-// Up to eight elements at the end of a row: `n` of them exist, the others read as zero and are not written.
+// Up to eight elements at the end of a row: `n` >= 1 of them exist, the others read as zero and are not written.  (The last
+// one is loaded again in their place, so that all loads are in flight at once; a branch around each would wait for each.)
 template <int DT>
 __device__ __forceinline__ typename Elem<DT>::Raw load_some(const typename Elem<DT>::type* p, int64_t n) {
   if (n >= 8) return Elem<DT>::load(p);
   float f[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) f[i] = i < n ? Elem<DT>::get(p[i]) : 0.0f;
+  for (int i = 0; i < 8; ++i) f[i] = Elem<DT>::get(p[i < n ? i : (int)n - 1]);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = i < n ? f[i] : 0.0f;
   return Elem<DT>::pack(f);
 }
 template <int DT>

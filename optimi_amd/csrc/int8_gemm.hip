@@ -56,51 +56,96 @@ __device__ __forceinline__ Tile tile_of(int id, int rows, int cols) {
   return {first + in % height, in / height};
 }
 
-// The steps [begin, end) of a sum over two pairs of tiles in LDS: while one is multiplied, the next step's is on its
-// way.  fetch<which>(step) starts the loads, settle<which>() finishes them and lets the workgroup meet, multiply<which>()
-// adds the tile's products.  The last step's tile may end anywhere, so it has a fetch of its own that looks at every
-// border, and its products leave out what is not there; the others' fetch needs no care.  The last step works on the first
-// pair of tiles, and which pair the first step takes follows from that; the second pair is free when the sums are done.
+// The steps [begin, end) of a sum over two pairs of tiles in LDS, copied there asynchronously: while one pair is multiplied, the
+// next step's copies are on their way.  fetch(step, which) starts them, multiply(which, last) adds a pair's products;
+// the last step works on the first pair, so that the second is free when the sums are done.
 template <int I>
 using Pair = std::integral_constant<int, I>;
-template <class Fetch, class FetchLast, class Settle, class Multiply, class MultiplyLast>
-__device__ __forceinline__ void run_steps(int begin, int end, Fetch fetch, FetchLast fetch_last, Settle settle, Multiply multiply, MultiplyLast multiply_last) {
+template <class Fetch, class Multiply>
+__device__ __forceinline__ void run_copied(int begin, int end, Fetch fetch, Multiply multiply) {
   const Pair<0> p0;
   const Pair<1> p1;
+  const std::false_type more;
   if (begin >= end) return;
-  if (end - begin == 1) {
-    fetch_last(begin, p0);
-    settle(p0);
-    multiply_last(p0);
-    return;
-  }
   int step = begin;
   if ((end - begin) % 2) {
     fetch(step, p0);
-    settle(p0);
-    fetch(++step, p1);
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(p0);
-    settle(p1);
+    meet();
   } else {
     fetch(step, p1);
-    settle(p1);
+    meet();
+    fetch(++step, p0);
+    __builtin_amdgcn_sched_barrier(0);  // the copies start before the products do; left alone, they are moved behind them
+    multiply(p1, more);
+    meet();
   }
-  for (; step + 2 < end; step += 2) {
-    fetch(step + 1, p0);
-    __builtin_amdgcn_sched_barrier(0);  // the loads start before the products do; left alone, they are moved behind them
-    multiply(p1);
-    settle(p0);
-    fetch(step + 2, p1);
+  for (; step + 1 < end; step += 2) {
+    fetch(step + 1, p1);
     __builtin_amdgcn_sched_barrier(0);
-    multiply(p0);
-    settle(p1);
+    multiply(p0, more);
+    meet();
+    fetch(step + 2, p0);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(p1, more);
+    meet();
   }
-  fetch_last(end - 1, p0);
-  __builtin_amdgcn_sched_barrier(0);
-  multiply(p1);
-  settle(p0);
-  multiply_last(p0);
+  multiply(p0, std::true_type{});
+}
+
+// The same through registers, which can be loaded from any address: load(step, part, last) starts the loads of a step that is two
+// ahead, write(which, part) brings a part that has arrived to LDS, multiply(which, more, part) adds a pair's products
+// and, with `more`, does what write() does to the other pair on the way.  Only the last step's loads look at the matrices'
+// borders, and they are not told apart inside the loop: a branch around loads makes the compiler wait for all of them in
+// front of the next ones.
+template <class Part, class Load, class Write, class Multiply>
+__device__ __forceinline__ void run_loaded(int begin, int end, Part (&part)[2], Load load, Write write, Multiply multiply) {
+  const Pair<0> p0;
+  const Pair<1> p1;
+  const std::false_type ordinary, no_more;
+  const std::true_type last, more;
+  auto loaded_step = [&](int step, auto which, auto is_last) OPTIMI_INLINE {
+    constexpr int W = decltype(which)::value;
+    load(step + 2, part[W], is_last);
+    __builtin_amdgcn_sched_barrier(0);
+    multiply(which, more, part[1 - W]);
+    __syncthreads();
+  };
+  const int n = end - begin;
+  if (n <= 0) return;
+  if (n == 1) {
+    load(begin, part[0], last);
+    write(p0, part[0]);
+    __syncthreads();
+  } else {
+    if (n == 2) {
+      load(begin, part[1], ordinary);
+      load(begin + 1, part[0], last);
+      write(p1, part[1]);
+      __syncthreads();
+    } else {
+      int step = begin;
+      if (n % 2) {
+        load(step, part[0], ordinary);
+        load(step + 1, part[1], ordinary);
+        write(p0, part[0]);
+        __syncthreads();
+      } else {
+        load(step, part[1], ordinary);
+        load(step + 1, part[0], ordinary);
+        write(p1, part[1]);
+        __syncthreads();
+        loaded_step(step++, p1, ordinary);
+      }
+      for (; step + 3 < end; step += 2) {
+        loaded_step(step, p0, ordinary);
+        loaded_step(step + 1, p1, ordinary);
+      }
+      loaded_step(step, p0, last);
+    }
+    multiply(p1, more, part[0]);
+    __syncthreads();
+  }
+  multiply(p0, no_more, part[0]);
 }
 
 // A wave's way from the matrix instruction's layout to rows: R rows of C 32-bit results in LDS, in pieces of four;
@@ -141,13 +186,21 @@ struct MatmulArgs {
   int steps_per_split;
 };
 
-// 16 bytes of a row from byte k on; what lies behind the row's end reads as zero.
+// 16 bytes of a row from byte k < len on; what lies behind the row's end reads as zero.  At the end the bytes are loaded one
+// by one, the last one again in place of those that are not there: sixteen loads in flight, where a branch around each
+// would wait for each.
 __device__ __forceinline__ u32x4 load_bytes(const int8_t* row, int64_t k, int64_t len) {
   if (k + 16 <= len) return *(const u32x4_align1*)(row + k);
-  u32x4 v{0, 0, 0, 0};
+  const int some = (int)(len - k);
+  uint32_t byte[16];
 #pragma unroll
-  for (int i = 0; i < 16; ++i)
-    if (k + i < len) v[i / 4] |= (uint32_t)(uint8_t)row[k + i] << (8 * (i % 4));
+  for (int i = 0; i < 16; ++i) byte[i] = (uint8_t)row[k + (i < some ? i : some - 1)];
+  u32x4 v;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const uint32_t word = byte[4 * w] | byte[4 * w + 1] << 8 | byte[4 * w + 2] << 16 | byte[4 * w + 3] << 24;
+    v[w] = some >= 4 * w + 4 ? word : some <= 4 * w ? 0u : word & ((1u << (8 * (some - 4 * w))) - 1u);
+  }
   return v;
 }
 
@@ -313,46 +366,59 @@ struct MatmulTile {
   }
 };
 
-// Two pairs of tiles in LDS.  ALIGNED: rows start on 16 bytes.
-template <int DT, int BM, int BN, int WM, int WN, bool ALIGNED>
+// Rows that start on 16 bytes: two pairs of tiles in LDS.
+template <int DT, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(WM * WN * 64) matmul_kernel(MatmulArgs p) {
   using M = MatmulTile<DT, BM, BN, WM, WN>;
   using TA = typename M::TA;
   using TB = typename M::TB;
   __shared__ __attribute__((aligned(1024))) int8_t a0[BM * kStep], a1[BM * kStep], b0[BN * kStep], b1[BN * kStep];
   M tile(p);
-  u32x4 va[TA::kPieces], vb[TB::kPieces];
+  const uint32_t len = (uint32_t)p.k;
+  const Buffer ra = buffer_of(tile.a(), tile.rows_a() * p.k), rb = buffer_of(tile.b(), tile.rows_b() * p.k);
+  run_copied(
+      tile.begin, tile.end,
+      [&](int step, auto which) OPTIMI_INLINE {
+        TA::copy(ra, len, step * kStep, which.value ? a1 : a0);
+        TB::copy(rb, len, step * kStep, which.value ? b1 : b0);
+      },
+      [&](auto which, auto last) OPTIMI_INLINE { tile.template multiply<last.value>(which.value ? a1 : a0, which.value ? b1 : b0); });
+  // the second pair of tiles is free
+  static_assert(M::kWaves / 2 * M::O::kBytes <= BM * kStep && M::kWaves / 2 * M::O::kBytes <= BN * kStep, "half of the waves' blocks fit either tile");
+  tile.store((uint32_t*)((tile.wave < M::kWaves / 2 ? a1 : b1) + tile.wave % (M::kWaves / 2) * M::O::kBytes));
+}
+
+// Rows that start anywhere.
+template <int DT, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__(WM * WN * 64) matmul_loaded_kernel(MatmulArgs p) {
+  using M = MatmulTile<DT, BM, BN, WM, WN>;
+  using TA = typename M::TA;
+  using TB = typename M::TB;
+  __shared__ __attribute__((aligned(1024))) int8_t a0[BM * kStep], a1[BM * kStep], b0[BN * kStep], b1[BN * kStep];
+  M tile(p);
+  struct Part {
+    u32x4 a[TA::kPieces], b[TB::kPieces];
+  };
+  Part part[2];
   const int rows_a = tile.rows_a(), rows_b = tile.rows_b();
   const uint32_t len = (uint32_t)p.k;
-  const Buffer ra = buffer_of(tile.a(), rows_a * p.k), rb = buffer_of(tile.b(), rows_b * p.k);
-  auto fetch = [&](int step, auto which) OPTIMI_INLINE {
-    if constexpr (ALIGNED) {
-      TA::copy(ra, len, step * kStep, which.value ? a1 : a0);
-      TB::copy(rb, len, step * kStep, which.value ? b1 : b0);
+  auto load = [&](int step, Part& v, auto last) OPTIMI_INLINE {
+    if constexpr (last.value) {
+      TA::load_last(tile.a(), rows_a, len, step * kStep, v.a);
+      TB::load_last(tile.b(), rows_b, len, step * kStep, v.b);
     } else {
-      TA::load(tile.a(), rows_a, len, step * kStep, va);
-      TB::load(tile.b(), rows_b, len, step * kStep, vb);
+      TA::load(tile.a(), rows_a, len, step * kStep, v.a);
+      TB::load(tile.b(), rows_b, len, step * kStep, v.b);
     }
   };
-  auto fetch_last = [&](int step, auto which) OPTIMI_INLINE {
-    if constexpr (ALIGNED) {
-      fetch(step, which);
-    } else {
-      TA::load_last(tile.a(), rows_a, len, step * kStep, va);
-      TB::load_last(tile.b(), rows_b, len, step * kStep, vb);
-    }
+  auto write = [&](auto which, const Part& v) OPTIMI_INLINE {
+    TA::store(v.a, which.value ? a1 : a0);
+    TB::store(v.b, which.value ? b1 : b0);
   };
-  auto settle = [&](auto which) OPTIMI_INLINE {
-    if constexpr (!ALIGNED) {
-      TA::store(va, which.value ? a1 : a0);
-      TB::store(vb, which.value ? b1 : b0);
-    }
-    meet();
-  };
-  run_steps(tile.begin, tile.end, fetch, fetch_last, settle,
-            [&](auto which) OPTIMI_INLINE { tile.template multiply<false>(which.value ? a1 : a0, which.value ? b1 : b0); },
-            [&](auto which) OPTIMI_INLINE { tile.template multiply<true>(which.value ? a1 : a0, which.value ? b1 : b0); });
-  // the second pair of tiles is free
+  run_loaded(tile.begin, tile.end, part, load, write, [&](auto which, auto more, const Part& v) OPTIMI_INLINE {
+    tile.template multiply<false>(which.value ? a1 : a0, which.value ? b1 : b0);
+    if (more.value) write(Pair<1 - which.value>{}, v);
+  });
   static_assert(M::kWaves / 2 * M::O::kBytes <= BM * kStep && M::kWaves / 2 * M::O::kBytes <= BN * kStep, "half of the waves' blocks fit either tile");
   tile.store((uint32_t*)((tile.wave < M::kWaves / 2 ? a1 : b1) + tile.wave % (M::kWaves / 2) * M::O::kBytes));
 }
@@ -792,7 +858,9 @@ __global__ void __launch_bounds__(512) weight_grad_kernel(WeightGradArgs p) {
       }
     }
   };
-  auto multiply = [&](const short* g, const short* q, auto more, const Part& v, short* next_g, short* next_q) OPTIMI_INLINE {
+  auto multiply = [&](auto which, auto more, const Part& v) OPTIMI_INLINE {
+    const short *g = which.value ? g1 : g0, *q = which.value ? q1 : q0;
+    short *next_g = which.value ? g0 : g1, *next_q = which.value ? q0 : q1;
     s16x8 fq[2][kC], fg[3];
     Turn t;
     auto read_g = [&](int at) OPTIMI_INLINE {  // the smallest pieces first
@@ -817,58 +885,14 @@ __global__ void __launch_bounds__(512) weight_grad_kernel(WeightGradArgs p) {
     }
     if (more.value) turn_special(v, t, next_g);
   };
-  // One step, with the loads of the next but one: an ordinary step's, the last one's, or none.  They are not told apart inside
-  // the loop: a branch around loads makes the compiler wait for all of them in front of the next ones.
-  const std::false_type ordinary;
-  const std::true_type last;
-  auto step_on = [&](int step, auto which, auto loads) OPTIMI_INLINE {
-    constexpr int W = decltype(which)::value;
-    loads(step + 2, part[W]);
-    __builtin_amdgcn_sched_barrier(0);
-    multiply(W ? g1 : g0, W ? q1 : q0, std::true_type{}, part[1 - W], W ? g0 : g1, W ? q0 : q1);
-    __syncthreads();
-  };
-  auto load_next = [&](int step, Part& v) OPTIMI_INLINE { load(step, v, ordinary); };
-  auto load_last = [&](int step, Part& v) OPTIMI_INLINE { load(step, v, last); };
-  auto load_none = [&](int, Part&) OPTIMI_INLINE {};
-  auto start = [&](auto which) OPTIMI_INLINE {
-    constexpr int W = decltype(which)::value;
-    Turn t;
+  run_loaded(begin, end, part, load,
+             [&](auto which, const Part& v) OPTIMI_INLINE {
+               Turn t;
 #pragma unroll
-    for (int at = 0; at < kGroups; ++at) turn(at, part[W], t, W ? g1 : g0, W ? q1 : q0);
-    turn_special(part[W], t, W ? g1 : g0);
-    __syncthreads();
-  };
-  const Pair<0> p0;
-  const Pair<1> p1;
-  const int n = end - begin;  // the last step works on the first pair of tiles
-  if (n == 1) {
-    load(begin, part[0], last);
-    start(p0);
-  } else if (n == 2) {
-    load(begin, part[1], ordinary);
-    load(begin + 1, part[0], last);
-    start(p1);
-  } else if (n > 2) {
-    int step = begin;
-    if (n % 2) {
-      load(step, part[0], ordinary);
-      load(step + 1, part[1], ordinary);
-      start(p0);
-    } else {
-      load(step, part[1], ordinary);
-      load(step + 1, part[0], ordinary);
-      start(p1);
-      step_on(step++, p1, load_next);
-    }
-    for (; step + 3 < end; step += 2) {
-      step_on(step, p0, load_next);
-      step_on(step + 1, p1, load_next);
-    }
-    step_on(step++, p0, load_last);
-  }
-  if (n > 1) step_on(end - 2, p1, load_none);
-  if (n > 0) multiply(g0, q0, std::false_type{}, part[0], g1, q1);
+               for (int at = 0; at < kGroups; ++at) turn(at, v, t, which.value ? g1 : g0, which.value ? q1 : q0);
+               turn_special(v, t, which.value ? g1 : g0);
+             },
+             multiply);
 
   using O = OutBlock<16, 32>;
   static_assert(kWaves / 2 * O::kBytes <= kPlane * 2, "half of the waves' blocks fit a tile");
@@ -1266,12 +1290,12 @@ int optimi_hip_int8_matmul(const int8_t* a, const float* a_scales, const int8_t*
     constexpr int DT = decltype(dt)::value;
     const dim3 grid((unsigned)(c.tiles * c.splits));
     if (c.tile == 256) {
-      matmul_kernel<DT, 256, 256, 2, 4, true><<<grid, dim3(512), 0, stream>>>(args);
+      matmul_kernel<DT, 256, 256, 2, 4><<<grid, dim3(512), 0, stream>>>(args);
     } else if (c.tile == 128) {
-      matmul_kernel<DT, 128, 128, 2, 2, true><<<grid, dim3(256), 0, stream>>>(args);
+      matmul_kernel<DT, 128, 128, 2, 2><<<grid, dim3(256), 0, stream>>>(args);
     } else {
       if (aligned) matmul_deep_kernel<DT, 64, 64, 2, 2><<<grid, dim3(256), 0, stream>>>(args);
-      else matmul_kernel<DT, 64, 64, 2, 2, false><<<grid, dim3(256), 0, stream>>>(args);
+      else matmul_loaded_kernel<DT, 64, 64, 2, 2><<<grid, dim3(256), 0, stream>>>(args);
     }
     OPTIMI_INT8_TRY(hipGetLastError());
     if (c.splits > 1) {

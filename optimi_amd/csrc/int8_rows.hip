@@ -14,9 +14,11 @@ namespace {
 
 using namespace optimi_int8;
 
-constexpr int kBlock = 256;           // lanes of a workgroup; 256 / TEAM rows are in work at once
-constexpr int kWaveRowCols = 1024;    // rows up to here belong to one wavefront: no LDS, no barrier
-constexpr int kLongCols = 8 * kBlock * 8;  // rows beyond 16384 elements do not stay in registers
+constexpr int kBlock = 256;         // lanes of a workgroup, or TEAM where that is more
+constexpr int kWaveRowCols = 1024;  // rows up to here belong to one wavefront: no LDS, no barrier
+constexpr int kLongCols = 16384;    // rows beyond do not stay in registers
+template <int TEAM>
+constexpr int kLanes = TEAM > kBlock ? TEAM : kBlock;
 
 // Grids stay far below the 2^32 threads that a launch may have; a workgroup takes further rows in a loop.
 constexpr int64_t kMaxBlocks = 1 << 20;
@@ -33,16 +35,45 @@ struct Place {
   int64_t step; // rows that the whole grid takes at once
   __device__ __forceinline__ Place() {
     lane = threadIdx.x % TEAM;
-    row = (int64_t)blockIdx.x * (kBlock / TEAM) + threadIdx.x / TEAM;
-    step = (int64_t)gridDim.x * (kBlock / TEAM);
+    row = (int64_t)blockIdx.x * (kLanes<TEAM> / TEAM) + __builtin_amdgcn_readfirstlane((int)threadIdx.x / TEAM);
+    step = (int64_t)gridDim.x * (kLanes<TEAM> / TEAM);
   }
 };
 
+// The eight elements from c on of a row.  Where the row ends inside of them, the vector is the row's last eight elements: some
+// of them are the neighbour's too, which computes and stores the same for them, so a row of any width takes whole
+// vectors only, without a branch.  A row of less than eight elements (TINY) is the exception.
+__device__ __forceinline__ int place8(int c, int cols) { return c + 8 <= cols ? c : cols - 8; }
+template <int DT, bool TINY>
+__device__ __forceinline__ typename Elem<DT>::Raw load8(const typename Elem<DT>::type* row, int c, int cols) {
+  if (TINY && cols < 8) return load_some<DT>(row, cols);
+  return Elem<DT>::load(row + place8(c, cols));
+}
+template <int DT, bool TINY>
+__device__ __forceinline__ void store8(typename Elem<DT>::type* row, int c, int cols, const float (&f)[8]) {
+  if (TINY && cols < 8) store_some<DT>(row, f, cols);
+  else Elem<DT>::store(row + place8(c, cols), Elem<DT>::pack(f));
+}
+template <bool TINY>
+__device__ __forceinline__ void store_values8(int8_t* row, int c, int cols, u32x2 v) {
+  if (TINY && cols < 8) store_values(row, v, cols);
+  else store_values(row + place8(c, cols), v, 8);
+}
+// For sums: the elements that the neighbour has as well count once.
+template <bool TINY>
+__device__ __forceinline__ void once(float (&f)[8], int c, int cols) {
+  if (cols % 8 == 0 || (TINY && cols < 8)) return;
+  const int skip = c - place8(c, cols);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = i < skip ? 0.0f : f[i];
+}
+
 template <int DT, int TEAM, int VPT>
-__global__ void __launch_bounds__(kBlock) quantize_kernel(const typename Elem<DT>::type* __restrict__ x, int64_t rows, int64_t cols,
+__global__ void __launch_bounds__(kLanes<TEAM>) quantize_kernel(const typename Elem<DT>::type* __restrict__ x, int64_t rows, int cols,
                                                           int8_t* __restrict__ values, float* __restrict__ scales) {
   using E = Elem<DT>;
-  __shared__ uint32_t slots[2][kBlock / 64];
+  constexpr bool kTiny = TEAM == 64 && VPT == 1;
+  __shared__ uint32_t slots[2][kLanes<TEAM> / 64];
   const Place<TEAM> at;
   // a team of four waves has the workgroup to itself, so all of its waves make the same number of rounds
   int turn = 0;
@@ -52,8 +83,9 @@ __global__ void __launch_bounds__(kBlock) quantize_kernel(const typename Elem<DT
     uint32_t most = 0;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      const int64_t c = (int64_t)(v * TEAM + at.lane) * 8;
-      raw[v] = c < cols ? load_some<DT>(in + c, cols - c) : E::zero();
+      const int c = (v * TEAM + at.lane) * 8;
+      raw[v] = E::zero();
+      if (c < cols) raw[v] = load8<DT, kTiny>(in, c, cols);
     }
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
@@ -66,10 +98,10 @@ __global__ void __launch_bounds__(kBlock) quantize_kernel(const typename Elem<DT
     const RowScale s = row_scale<DT>(most);
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      const int64_t c = (int64_t)(v * TEAM + at.lane) * 8;
+      const int c = (v * TEAM + at.lane) * 8;
       float f[8];
       E::unpack(raw[v], f);
-      if (c < cols) store_values(values + row * cols + c, quantize8(f, s), cols - c);
+      if (c < cols) store_values8<kTiny>(values + row * cols, c, cols, quantize8(f, s));
     }
     if (at.lane == 0) scales[row] = s.scale;
   }
@@ -77,7 +109,7 @@ __global__ void __launch_bounds__(kBlock) quantize_kernel(const typename Elem<DT
 
 // Rows that do not fit the registers: one workgroup each, read twice.
 template <int DT>
-__global__ void __launch_bounds__(kBlock) quantize_long_kernel(const typename Elem<DT>::type* __restrict__ x, int64_t rows, int64_t cols,
+__global__ void __launch_bounds__(kBlock) quantize_long_kernel(const typename Elem<DT>::type* __restrict__ x, int64_t rows, int cols,
                                                                int8_t* __restrict__ values, float* __restrict__ scales) {
   using E = Elem<DT>;
   __shared__ uint32_t slots[2][kBlock / 64];
@@ -85,18 +117,18 @@ __global__ void __launch_bounds__(kBlock) quantize_long_kernel(const typename El
   for (int64_t row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
     const typename E::type* in = x + row * cols;
     uint32_t most = 0;
-    for (int64_t c = (int64_t)threadIdx.x * 8; c < cols; c += kBlock * 8) {
+    for (int c = threadIdx.x * 8; c < cols; c += kBlock * 8) {
       float f[8];
-      E::unpack(load_some<DT>(in + c, cols - c), f);
+      E::unpack(load8<DT, false>(in, c, cols), f);
 #pragma unroll
       for (int i = 0; i < 8; ++i) most = MaxOp::join(most, abs_bits(f[i]));
     }
     most = team_reduce<MaxOp, kBlock>(most, slots[turn]);
     const RowScale s = row_scale<DT>(most);
-    for (int64_t c = (int64_t)threadIdx.x * 8; c < cols; c += kBlock * 8) {
+    for (int c = threadIdx.x * 8; c < cols; c += kBlock * 8) {
       float f[8];
-      E::unpack(load_some<DT>(in + c, cols - c), f);
-      store_values(values + row * cols + c, quantize8(f, s), cols - c);
+      E::unpack(load8<DT, false>(in, c, cols), f);
+      store_values8<false>(values + row * cols, c, cols, quantize8(f, s));
     }
     if (threadIdx.x == 0) scales[row] = s.scale;
   }
@@ -105,22 +137,22 @@ __global__ void __launch_bounds__(kBlock) quantize_long_kernel(const typename El
 // q * s, eight values a lane; `team` lanes (a power of two) share a row.
 template <int DT>
 __global__ void __launch_bounds__(kBlock) dequantize_kernel(const int8_t* __restrict__ values, const float* __restrict__ scales, int64_t rows,
-                                                            int64_t cols, int team, typename Elem<DT>::type* __restrict__ out) {
+                                                            int cols, int team, typename Elem<DT>::type* __restrict__ out) {
   const int lane = threadIdx.x % team;
   for (int64_t row = (int64_t)blockIdx.x * (kBlock / team) + threadIdx.x / team; row < rows; row += (int64_t)gridDim.x * (kBlock / team)) {
     const float s = scales[row];
-    for (int64_t c = (int64_t)lane * 8; c < cols; c += team * 8) {
-      const int8_t* p = values + row * cols + c;
+    const int8_t* from = values + row * cols;
+    for (int c = lane * 8; c < cols; c += team * 8) {
       float f[8];
-      if (cols - c >= 8) {
-        const u32x2 q = *(const u32x2_align1*)p;
+      if (cols >= 8) {
+        const u32x2 q = *(const u32x2_align1*)(from + place8(c, cols));
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] = (float)(int8_t)(q[i / 4] >> (8 * (i % 4))) * s;
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = i < cols - c ? (float)p[i] * s : 0.0f;
+        for (int i = 0; i < 8; ++i) f[i] = (float)from[i < cols ? i : 0] * s;
       }
-      store_some<DT>(out + row * cols + c, f, cols - c);
+      store8<DT, true>(out + row * cols, c, cols, f);
     }
   }
 }
@@ -130,8 +162,9 @@ template <int DT, bool W32>
 struct Weight {
   static constexpr int kType = W32 ? (int)OPTIMI_F32 : DT;
   using E = Elem<kType>;
-  static __device__ __forceinline__ void load(const void* w, int64_t c, int64_t cols, float (&f)[8]) {
-    E::unpack(load_some<kType>((const typename E::type*)w + c, cols - c), f);
+  template <bool TINY>
+  static __device__ __forceinline__ void load(const void* w, int c, int cols, float (&f)[8]) {
+    E::unpack(load8<kType, TINY>((const typename E::type*)w, c, cols), f);
   }
 };
 
@@ -149,7 +182,8 @@ __device__ __forceinline__ typename Elem<DT>::Raw add_rows(const typename Elem<D
 
 struct NormArgs {
   const void *x, *residual, *weight;
-  int64_t rows, cols;
+  int64_t rows;
+  int cols;
   float eps;
   void* h;
   int8_t* values;
@@ -161,29 +195,32 @@ __device__ __forceinline__ float inverse_rms(float sum_of_squares, int64_t cols,
 }
 
 template <int DT, bool W32, int TEAM, int VPT>
-__global__ void __launch_bounds__(kBlock) norm_kernel(NormArgs a) {
+__global__ void __launch_bounds__(kLanes<TEAM>) norm_kernel(NormArgs a) {
   using E = Elem<DT>;
   using T = typename E::type;
-  __shared__ uint32_t slots[2][2][kBlock / 64];
+  constexpr bool kTiny = TEAM == 64 && VPT == 1;
+  __shared__ uint32_t slots[2][2][kLanes<TEAM> / 64];
   const Place<TEAM> at;
+  const int cols = a.cols;
   int turn = 0;
   for (int64_t row = at.row; row < a.rows; row += at.step, turn ^= 1) {
     typename E::Raw raw[VPT];
     float sum = 0.0f;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      const int64_t c = (int64_t)(v * TEAM + at.lane) * 8;
-      raw[v] = c < a.cols ? load_some<DT>((const T*)a.x + row * a.cols + c, a.cols - c) : E::zero();
+      const int c = (v * TEAM + at.lane) * 8;
+      raw[v] = E::zero();
+      if (c < cols) raw[v] = load8<DT, kTiny>((const T*)a.x + row * cols, c, cols);
     }
     if (a.residual) {
 #pragma unroll
       for (int v = 0; v < VPT; ++v) {
-        const int64_t c = (int64_t)(v * TEAM + at.lane) * 8;
-        if (c < a.cols) {
-          raw[v] = add_rows<DT>(raw[v], load_some<DT>((const T*)a.residual + row * a.cols + c, a.cols - c));
+        const int c = (v * TEAM + at.lane) * 8;
+        if (c < cols) {
+          raw[v] = add_rows<DT>(raw[v], load8<DT, kTiny>((const T*)a.residual + row * cols, c, cols));
           float f[8];
           E::unpack(raw[v], f);
-          store_some<DT>((T*)a.h + row * a.cols + c, f, a.cols - c);
+          store8<DT, kTiny>((T*)a.h + row * cols, c, cols, f);
         }
       }
     }
@@ -191,20 +228,21 @@ __global__ void __launch_bounds__(kBlock) norm_kernel(NormArgs a) {
     for (int v = 0; v < VPT; ++v) {
       float f[8];
       E::unpack(raw[v], f);
+      once<kTiny>(f, (v * TEAM + at.lane) * 8, cols);
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum = fmaf(f[i], f[i], sum);
     }
     sum = __uint_as_float(team_reduce<SumOp, TEAM>(__float_as_uint(sum), slots[turn][0]));
-    const float r = inverse_rms(sum, a.cols, a.eps);
+    const float r = inverse_rms(sum, cols, a.eps);
     uint32_t most = 0;
     float y[VPT][8];
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      const int64_t c = (int64_t)(v * TEAM + at.lane) * 8;
+      const int c = (v * TEAM + at.lane) * 8;
       float f[8], w[8];
       E::unpack(raw[v], f);
-      if (c < a.cols) {
-        Weight<DT, W32>::load(a.weight, c, a.cols, w);
+      if (c < cols) {
+        Weight<DT, W32>::template load<kTiny>(a.weight, c, cols, w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           y[v][i] = f[i] * r * w[i];
@@ -216,8 +254,8 @@ __global__ void __launch_bounds__(kBlock) norm_kernel(NormArgs a) {
     const RowScale s = row_scale<OPTIMI_F32>(most);
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      const int64_t c = (int64_t)(v * TEAM + at.lane) * 8;
-      if (c < a.cols) store_values(a.values + row * a.cols + c, quantize8(y[v], s), a.cols - c);
+      const int c = (v * TEAM + at.lane) * 8;
+      if (c < cols) store_values8<kTiny>(a.values + row * cols, c, cols, quantize8(y[v], s));
     }
     if (at.lane == 0) {
       a.scales[row] = s.scale;
@@ -231,42 +269,44 @@ __global__ void __launch_bounds__(kBlock) norm_long_kernel(NormArgs a) {
   using E = Elem<DT>;
   using T = typename E::type;
   __shared__ uint32_t slots[2][2][kBlock / 64];
+  const int cols = a.cols;
   int turn = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
-    const T* x = (const T*)a.x + row * a.cols;
-    const T* res = a.residual ? (const T*)a.residual + row * a.cols : nullptr;
-    auto kept = [&](int64_t c, float (&f)[8]) {  // h, formed again from its two terms wherever it is needed
-      typename E::Raw raw = load_some<DT>(x + c, a.cols - c);
-      if (res) raw = add_rows<DT>(raw, load_some<DT>(res + c, a.cols - c));
+    const T* x = (const T*)a.x + row * cols;
+    const T* res = a.residual ? (const T*)a.residual + row * cols : nullptr;
+    auto kept = [&](int c, float (&f)[8]) {  // h, formed again from its two terms wherever it is needed
+      typename E::Raw raw = load8<DT, false>(x, c, cols);
+      if (res) raw = add_rows<DT>(raw, load8<DT, false>(res, c, cols));
       E::unpack(raw, f);
     };
     float sum = 0.0f;
-    for (int64_t c = (int64_t)threadIdx.x * 8; c < a.cols; c += kBlock * 8) {
+    for (int c = threadIdx.x * 8; c < cols; c += kBlock * 8) {
       float f[8];
       kept(c, f);
+      once<false>(f, c, cols);
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum = fmaf(f[i], f[i], sum);
     }
     sum = __uint_as_float(team_reduce<SumOp, kBlock>(__float_as_uint(sum), slots[turn][0]));
-    const float r = inverse_rms(sum, a.cols, a.eps);
+    const float r = inverse_rms(sum, cols, a.eps);
     uint32_t most = 0;
-    for (int64_t c = (int64_t)threadIdx.x * 8; c < a.cols; c += kBlock * 8) {
+    for (int c = threadIdx.x * 8; c < cols; c += kBlock * 8) {
       float f[8], w[8];
       kept(c, f);
-      Weight<DT, W32>::load(a.weight, c, a.cols, w);
+      Weight<DT, W32>::template load<false>(a.weight, c, cols, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) most = MaxOp::join(most, abs_bits(f[i] * r * w[i]));
     }
     most = team_reduce<MaxOp, kBlock>(most, slots[turn][1]);
     const RowScale s = row_scale<OPTIMI_F32>(most);
-    for (int64_t c = (int64_t)threadIdx.x * 8; c < a.cols; c += kBlock * 8) {
+    for (int c = threadIdx.x * 8; c < cols; c += kBlock * 8) {
       float f[8], w[8], y[8];
       kept(c, f);
-      Weight<DT, W32>::load(a.weight, c, a.cols, w);
+      Weight<DT, W32>::template load<false>(a.weight, c, cols, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] = f[i] * r * w[i];
-      store_values(a.values + row * a.cols + c, quantize8(y, s), a.cols - c);
-      if (res) store_some<DT>((T*)a.h + row * a.cols + c, f, a.cols - c);
+      store_values8<false>(a.values + row * cols, c, cols, quantize8(y, s));
+      if (res) store8<DT, false>((T*)a.h + row * cols, c, cols, f);
     }
     if (threadIdx.x == 0) {
       a.scales[row] = s.scale;
@@ -283,24 +323,27 @@ __global__ void __launch_bounds__(kBlock) norm_long_kernel(NormArgs a) {
 struct NormBackwardArgs {
   const void *grad, *grad_h, *h, *weight;
   const float* rstd;
-  int64_t rows, cols;
+  int64_t rows;
+  int cols;
   void* dx;
   float* partial;  // [teams][cols]
 };
 
 template <int DT, bool W32, int TEAM, int VPT>
-__global__ void __launch_bounds__(kBlock) norm_backward_kernel(NormBackwardArgs a) {
+__global__ void __launch_bounds__(kLanes<TEAM>) norm_backward_kernel(NormBackwardArgs a) {
   using E = Elem<DT>;
   using T = typename E::type;
-  __shared__ uint32_t slots[2][kBlock / 64];
+  constexpr bool kTiny = TEAM == 64 && VPT == 1;
+  __shared__ uint32_t slots[2][kLanes<TEAM> / 64];
   const Place<TEAM> at;
+  const int cols = a.cols;
   float w[VPT][8], dw[VPT][8];
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
-    const int64_t c = (int64_t)(v * TEAM + at.lane) * 8;
+    const int c = (v * TEAM + at.lane) * 8;
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[v][i] = dw[v][i] = 0.0f;
-    if (c < a.cols) Weight<DT, W32>::load(a.weight, c, a.cols, w[v]);
+    if (c < cols) Weight<DT, W32>::template load<kTiny>(a.weight, c, cols, w[v]);
   }
   int turn = 0;
   for (int64_t row = at.row; row < a.rows; row += at.step, turn ^= 1) {
@@ -308,46 +351,50 @@ __global__ void __launch_bounds__(kBlock) norm_backward_kernel(NormBackwardArgs 
     const float r = a.rstd[row];
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      const int64_t c = (int64_t)(v * TEAM + at.lane) * 8;
+      const int c = (v * TEAM + at.lane) * 8;
       g[v] = h[v] = more[v] = E::zero();
-      if (c < a.cols) {
-        g[v] = load_some<DT>((const T*)a.grad + row * a.cols + c, a.cols - c);
-        h[v] = load_some<DT>((const T*)a.h + row * a.cols + c, a.cols - c);
-        if (a.grad_h) more[v] = load_some<DT>((const T*)a.grad_h + row * a.cols + c, a.cols - c);
+      if (c < cols) {
+        g[v] = load8<DT, kTiny>((const T*)a.grad + row * cols, c, cols);
+        h[v] = load8<DT, kTiny>((const T*)a.h + row * cols, c, cols);
+        if (a.grad_h) more[v] = load8<DT, kTiny>((const T*)a.grad_h + row * cols, c, cols);
       }
     }
     float dot = 0.0f;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       float fg[8], fh[8];
+      float gw[8];
       E::unpack(g[v], fg);
       E::unpack(h[v], fh);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float xhat = fh[i] * r;
-        dw[v][i] = fmaf(fg[i], xhat, dw[v][i]);
-        dot = fmaf(fg[i] * w[v][i], xhat, dot);
+        fh[i] *= r;
+        dw[v][i] = fmaf(fg[i], fh[i], dw[v][i]);
+        gw[i] = fg[i] * w[v][i];
       }
+      once<kTiny>(gw, (v * TEAM + at.lane) * 8, cols);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dot = fmaf(gw[i], fh[i], dot);
     }
     dot = __uint_as_float(team_reduce<SumOp, TEAM>(__float_as_uint(dot), slots[turn]));
-    const float mean = dot / (float)a.cols;
+    const float mean = dot / (float)cols;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      const int64_t c = (int64_t)(v * TEAM + at.lane) * 8;
+      const int c = (v * TEAM + at.lane) * 8;
       float fg[8], fh[8], fm[8], d[8];
       E::unpack(g[v], fg);
       E::unpack(h[v], fh);
       E::unpack(more[v], fm);
 #pragma unroll
       for (int i = 0; i < 8; ++i) d[i] = fmaf(r, fg[i] * w[v][i] - fh[i] * r * mean, fm[i]);
-      if (c < a.cols) store_some<DT>((T*)a.dx + row * a.cols + c, d, a.cols - c);
+      if (c < cols) store8<DT, kTiny>((T*)a.dx + row * cols, c, cols, d);
     }
   }
-  const int64_t team = (int64_t)blockIdx.x * (kBlock / TEAM) + threadIdx.x / TEAM;
+  const int64_t team = (int64_t)blockIdx.x * (kLanes<TEAM> / TEAM) + threadIdx.x / TEAM;
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
-    const int64_t c = (int64_t)(v * TEAM + at.lane) * 8;
-    if (c < a.cols) store_some<OPTIMI_F32>(a.partial + team * a.cols + c, dw[v], a.cols - c);
+    const int c = (v * TEAM + at.lane) * 8;
+    if (c < cols) store8<OPTIMI_F32, kTiny>(a.partial + team * cols, c, cols, dw[v]);
   }
 }
 
@@ -356,31 +403,33 @@ __global__ void __launch_bounds__(kBlock) norm_backward_long_kernel(NormBackward
   using E = Elem<DT>;
   using T = typename E::type;
   __shared__ uint32_t slots[2][kBlock / 64];
+  const int cols = a.cols;
   int turn = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x, turn ^= 1) {
-    const T* grad = (const T*)a.grad + row * a.cols;
-    const T* h = (const T*)a.h + row * a.cols;
+    const T* grad = (const T*)a.grad + row * cols;
+    const T* h = (const T*)a.h + row * cols;
     const float r = a.rstd[row];
     float dot = 0.0f;
-    for (int64_t c = (int64_t)threadIdx.x * 8; c < a.cols; c += kBlock * 8) {
+    for (int c = threadIdx.x * 8; c < cols; c += kBlock * 8) {
       float fg[8], fh[8], w[8];
-      E::unpack(load_some<DT>(grad + c, a.cols - c), fg);
-      E::unpack(load_some<DT>(h + c, a.cols - c), fh);
-      Weight<DT, W32>::load(a.weight, c, a.cols, w);
+      E::unpack(load8<DT, false>(grad, c, cols), fg);
+      E::unpack(load8<DT, false>(h, c, cols), fh);
+      Weight<DT, W32>::template load<false>(a.weight, c, cols, w);
+      once<false>(fg, c, cols);
 #pragma unroll
       for (int i = 0; i < 8; ++i) dot = fmaf(fg[i] * w[i], fh[i] * r, dot);
     }
     dot = __uint_as_float(team_reduce<SumOp, kBlock>(__float_as_uint(dot), slots[turn]));
-    const float mean = dot / (float)a.cols;
-    for (int64_t c = (int64_t)threadIdx.x * 8; c < a.cols; c += kBlock * 8) {
+    const float mean = dot / (float)cols;
+    for (int c = threadIdx.x * 8; c < cols; c += kBlock * 8) {
       float fg[8], fh[8], fm[8], w[8], d[8];
-      E::unpack(load_some<DT>(grad + c, a.cols - c), fg);
-      E::unpack(load_some<DT>(h + c, a.cols - c), fh);
-      E::unpack(a.grad_h ? load_some<DT>((const T*)a.grad_h + row * a.cols + c, a.cols - c) : E::zero(), fm);
-      Weight<DT, W32>::load(a.weight, c, a.cols, w);
+      E::unpack(load8<DT, false>(grad, c, cols), fg);
+      E::unpack(load8<DT, false>(h, c, cols), fh);
+      E::unpack(a.grad_h ? load8<DT, false>((const T*)a.grad_h + row * cols, c, cols) : E::zero(), fm);
+      Weight<DT, W32>::template load<false>(a.weight, c, cols, w);
 #pragma unroll
       for (int i = 0; i < 8; ++i) d[i] = fmaf(r, fg[i] * w[i] - fh[i] * r * mean, fm[i]);
-      store_some<DT>((T*)a.dx + row * a.cols + c, d, a.cols - c);
+      store8<DT, false>((T*)a.dx + row * cols, c, cols, d);
     }
   }
 }
@@ -390,9 +439,9 @@ __global__ void __launch_bounds__(kBlock) norm_backward_long_kernel(NormBackward
 // gridDim.y-th row and leaves a partial row.
 template <int DT, bool NORM>
 __global__ void __launch_bounds__(kBlock) column_partial_kernel(const typename Elem<DT>::type* __restrict__ x, const typename Elem<DT>::type* __restrict__ h,
-                                                                const float* __restrict__ rstd, int64_t rows, int64_t cols, float* __restrict__ partial) {
+                                                                const float* __restrict__ rstd, int64_t rows, int cols, float* __restrict__ partial) {
   using E = Elem<DT>;
-  const int64_t c = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * 8;
+  const int c = (blockIdx.x * kBlock + threadIdx.x) * 8;
   if (c >= cols) return;
   float sum[8];
 #pragma unroll
@@ -400,10 +449,10 @@ __global__ void __launch_bounds__(kBlock) column_partial_kernel(const typename E
 #pragma unroll 4
   for (int64_t row = blockIdx.y; row < rows; row += gridDim.y) {
     float f[8];
-    E::unpack(load_some<DT>(x + row * cols + c, cols - c), f);
+    E::unpack(load8<DT, true>(x + row * cols, c, cols), f);
     if constexpr (NORM) {
       float fh[8];
-      E::unpack(load_some<DT>(h + row * cols + c, cols - c), fh);
+      E::unpack(load8<DT, true>(h + row * cols, c, cols), fh);
       const float r = rstd[row];
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum[i] = fmaf(f[i], fh[i] * r, sum[i]);
@@ -412,28 +461,28 @@ __global__ void __launch_bounds__(kBlock) column_partial_kernel(const typename E
       for (int i = 0; i < 8; ++i) sum[i] += f[i];
     }
   }
-  store_some<OPTIMI_F32>(partial + (int64_t)blockIdx.y * cols + c, sum, cols - c);
+  store8<OPTIMI_F32, true>(partial + (int64_t)blockIdx.y * cols, c, cols, sum);
 }
 
-// Adds the partial rows: 32 columns a workgroup, its eight groups of 32 lanes take every eighth partial row.
+// Adds the partial rows: 32 columns a workgroup, its groups of 32 lanes each take every kJoin-th partial row.
+constexpr int kJoin = 32;  // as many groups as columns: see the end
 template <int OUT>
-__global__ void __launch_bounds__(kBlock) column_finish_kernel(const float* __restrict__ partial, int64_t parts, int64_t cols,
-                                                               typename Elem<OUT>::type* __restrict__ out) {
-  __shared__ float sums[8][33];
+__global__ void __launch_bounds__(32 * kJoin) column_finish_kernel(const float* __restrict__ partial, int64_t parts, int64_t cols,
+                                                                   typename Elem<OUT>::type* __restrict__ out) {
+  __shared__ float sums[kJoin][33];
   const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
   for (int64_t c0 = (int64_t)blockIdx.x * 32; c0 < cols; c0 += (int64_t)gridDim.x * 32) {
     float s = 0.0f;
     if (c0 + lane < cols) {
 #pragma unroll 8
-      for (int64_t p = group; p < parts; p += 8) s += partial[p * cols + c0 + lane];
+      for (int64_t p = group; p < parts; p += kJoin) s += partial[p * cols + c0 + lane];
     }
     sums[group][lane] = s;
     __syncthreads();
-    if (group == 0 && c0 + lane < cols) {
+    float sum = sums[lane][group];  // a group of lanes for each of the 32 columns
 #pragma unroll
-      for (int g = 1; g < 8; ++g) s += sums[g][lane];
-      out[c0 + lane] = Elem<OUT>::put(s);
-    }
+    for (int d = 16; d > 0; d /= 2) sum += __shfl_xor(sum, d, 32);
+    if (lane == 0 && c0 + group < cols) out[c0 + group] = Elem<OUT>::put(sum);
     __syncthreads();
   }
 }
@@ -463,8 +512,9 @@ int by_width(int64_t cols, F f) {
   OPTIMI_WIDTH(256, 2);
   OPTIMI_WIDTH(256, 3);
   OPTIMI_WIDTH(256, 4);
-  OPTIMI_WIDTH(256, 6);
-  return f(std::integral_constant<int, 256>{}, std::integral_constant<int, 8>{});
+  OPTIMI_WIDTH(512, 3);
+  static_assert(kLongCols == 512 * 8 * 4, "the widest row that stays in registers");
+  return f(std::integral_constant<int, 512>{}, std::integral_constant<int, 4>{});
 #undef OPTIMI_WIDTH
 }
 
@@ -487,7 +537,7 @@ int finish_columns(const float* partial, int64_t parts, int64_t cols, int dtype,
   if (cols == 0) return 0;
   return by_dtype(dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    column_finish_kernel<DT><<<dim3(blocks_for(cols, 32)), dim3(kBlock), 0, stream>>>(partial, parts, cols, (typename Elem<DT>::type*)out);
+    column_finish_kernel<DT><<<dim3(blocks_for(cols, 32)), dim3(32 * kJoin), 0, stream>>>(partial, parts, cols, (typename Elem<DT>::type*)out);
     OPTIMI_INT8_TRY(hipGetLastError());
     return 0;
   });
@@ -508,7 +558,7 @@ int column_sum(const void* x, int64_t rows, int64_t cols, int dtype, void* out, 
     using T = typename Elem<DT>::type;
     const unsigned stripes = (unsigned)((cols + kBlock * 8 - 1) / (kBlock * 8));
     if (parts > 0) {
-      column_partial_kernel<DT, false><<<dim3(stripes, (unsigned)parts), dim3(kBlock), 0, stream>>>((const T*)x, nullptr, nullptr, rows, cols, (float*)workspace);
+      column_partial_kernel<DT, false><<<dim3(stripes, (unsigned)parts), dim3(kBlock), 0, stream>>>((const T*)x, nullptr, nullptr, rows, (int)cols, (float*)workspace);
       OPTIMI_INT8_TRY(hipGetLastError());
     }
     return finish_columns((const float*)workspace, parts, cols, dtype, out, stream);
@@ -530,11 +580,11 @@ int optimi_hip_int8_quantize(const void* x, int64_t rows, int64_t cols, int dtyp
     constexpr int DT = decltype(dt)::value;
     using T = typename Elem<DT>::type;
     if (cols > kLongCols) {
-      quantize_long_kernel<DT><<<dim3(blocks_for(rows, 1)), dim3(kBlock), 0, stream>>>((const T*)x, rows, cols, values, scales);
+      quantize_long_kernel<DT><<<dim3(blocks_for(rows, 1)), dim3(kBlock), 0, stream>>>((const T*)x, rows, (int)cols, values, scales);
     } else {
       by_width(cols, [&](auto team, auto vpt) {
         quantize_kernel<DT, decltype(team)::value, decltype(vpt)::value>
-            <<<dim3(blocks_for(rows, rows_per_block(cols))), dim3(kBlock), 0, stream>>>((const T*)x, rows, cols, values, scales);
+            <<<dim3(blocks_for(rows, rows_per_block(cols))), dim3(kLanes<decltype(team)::value>), 0, stream>>>((const T*)x, rows, (int)cols, values, scales);
         return 0;
       });
     }
@@ -553,7 +603,7 @@ int optimi_hip_int8_dequantize(const int8_t* values, const float* scales, int64_
   while (team < kBlock && (int64_t)team * 8 < cols) team *= 2;
   return by_dtype(dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    dequantize_kernel<DT><<<dim3(blocks_for(rows, kBlock / team)), dim3(kBlock), 0, (hipStream_t)stream_>>>(values, scales, rows, cols, team,
+    dequantize_kernel<DT><<<dim3(blocks_for(rows, kBlock / team)), dim3(kBlock), 0, (hipStream_t)stream_>>>(values, scales, rows, (int)cols, team,
                                                                                                          (typename Elem<DT>::type*)out);
     OPTIMI_INT8_TRY(hipGetLastError());
     return 0;
@@ -573,7 +623,7 @@ int optimi_hip_add_rms_norm_int8(const void* x, const void* residual, const void
       !aligned_to(scales, 4) || !aligned_to(rstd, 4))
     return OPTIMI_ERR_ALIGN;
   hipStream_t stream = (hipStream_t)stream_;
-  const NormArgs args{x, residual, weight, rows, cols, (float)eps, h, values, scales, rstd};
+  const NormArgs args{x, residual, weight, rows, (int)cols, (float)eps, h, values, scales, rstd};
   return by_dtype(dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     auto with = [&](auto w32) {
@@ -582,7 +632,7 @@ int optimi_hip_add_rms_norm_int8(const void* x, const void* residual, const void
         norm_long_kernel<DT, W32><<<dim3(blocks_for(rows, 1)), dim3(kBlock), 0, stream>>>(args);
       } else {
         by_width(cols, [&](auto team, auto vpt) {
-          norm_kernel<DT, W32, decltype(team)::value, decltype(vpt)::value><<<dim3(blocks_for(rows, rows_per_block(cols))), dim3(kBlock), 0, stream>>>(args);
+          norm_kernel<DT, W32, decltype(team)::value, decltype(vpt)::value><<<dim3(blocks_for(rows, rows_per_block(cols))), dim3(kLanes<decltype(team)::value>), 0, stream>>>(args);
           return 0;
         });
       }
@@ -612,7 +662,7 @@ int optimi_hip_add_rms_norm_int8_backward(const void* grad, const void* grad_h, 
   hipStream_t stream = (hipStream_t)stream_;
   const int64_t parts = norm_partials(rows, cols);
   if (rows > 0) {
-    const NormBackwardArgs args{grad, grad_h, h, weight, rstd, rows, cols, dx, (float*)workspace};
+    const NormBackwardArgs args{grad, grad_h, h, weight, rstd, rows, (int)cols, dx, (float*)workspace};
     const int rc = by_dtype(dtype, [&](auto dt) {
       constexpr int DT = decltype(dt)::value;
       using T = typename Elem<DT>::type;
@@ -622,11 +672,11 @@ int optimi_hip_add_rms_norm_int8_backward(const void* grad, const void* grad_h, 
           norm_backward_long_kernel<DT, W32><<<dim3(blocks_for(rows, 1)), dim3(kBlock), 0, stream>>>(args);
           OPTIMI_INT8_TRY(hipGetLastError());
           const unsigned stripes = (unsigned)((cols + kBlock * 8 - 1) / (kBlock * 8));
-          column_partial_kernel<DT, true><<<dim3(stripes, (unsigned)parts), dim3(kBlock), 0, stream>>>((const T*)grad, (const T*)h, rstd, rows, cols, (float*)workspace);
+          column_partial_kernel<DT, true><<<dim3(stripes, (unsigned)parts), dim3(kBlock), 0, stream>>>((const T*)grad, (const T*)h, rstd, rows, (int)cols, (float*)workspace);
         } else {
           by_width(cols, [&](auto team, auto vpt) {
             norm_backward_kernel<DT, W32, decltype(team)::value, decltype(vpt)::value>
-                <<<dim3((unsigned)partial_blocks(rows, cols)), dim3(kBlock), 0, stream>>>(args);
+                <<<dim3((unsigned)partial_blocks(rows, cols)), dim3(kLanes<decltype(team)::value>), 0, stream>>>(args);
             return 0;
           });
         }
