@@ -32,7 +32,14 @@ inline bool aligned_to(const void* p, int64_t bytes) { return ((uintptr_t)p % (u
 
 // Eight consecutive elements as they lie in memory, and as floats.  The loads and stores are written for
 // addresses that are aligned to one element only: rows of an odd width start anywhere, gfx950 takes one
-// 16-byte access at any such address, and an aligned one loses nothing by it.
+// 16-byte access at any such address, and an aligned one loses nothing by it.  stream and stream_out are for data that has
+// left the caches before it is used again: what a row kernel reads once, and results larger than a cache, which
+// would push out what is still needed (int8 product 8192 x 11008 x 4096: 359 us with ordinary stores, 341 us with these;
+// restoring 16384 x 11008 values and quantizing them before: 201 us, 171 us).  Lines that two rows share must not be
+// streamed out: they would be written in parts (fp32 weight gradient 4096 x 1023: 43 us, 53 us), hence whole_lines.
+// (Where both kinds of a store stand in two branches, empty assembly keeps them apart: merged, they would lose the hint.)
+__host__ __device__ inline bool whole_lines(int64_t cols, int size) { return cols * size % 64 == 0; }
+
 template <int DT>
 struct Elem;
 
@@ -46,9 +53,16 @@ struct Elem<OPTIMI_F32> {
   static __device__ __forceinline__ float get(type v) { return v; }
   static __device__ __forceinline__ type put(float v) { return v; }
   static __device__ __forceinline__ Raw load(const type* p) { return {*(const vec*)p, *(const vec*)(p + 4)}; }
+  static __device__ __forceinline__ Raw stream(const type* p) { return {__builtin_nontemporal_load((const vec*)p), __builtin_nontemporal_load((const vec*)(p + 4))}; }
   static __device__ __forceinline__ void store(type* p, const Raw& r) {
     *(vec*)p = r.a;
     *(vec*)(p + 4) = r.b;
+  }
+  static __device__ __forceinline__ void stream_out(type* p, const Raw& r) {
+    asm volatile("");
+    __builtin_nontemporal_store(r.a, (vec*)p);
+    __builtin_nontemporal_store(r.b, (vec*)(p + 4));
+    asm volatile("");
   }
   static __device__ __forceinline__ Raw zero() { return {u32x4{0, 0, 0, 0}, u32x4{0, 0, 0, 0}}; }
   static __device__ __forceinline__ void unpack(const Raw& r, float (&f)[8]) {
@@ -81,7 +95,13 @@ struct Elem<OPTIMI_BF16> {
   static __device__ __forceinline__ float get(type v) { return (float)v; }
   static __device__ __forceinline__ type put(float v) { return (type)v; }
   static __device__ __forceinline__ Raw load(const type* p) { return {*(const u32x4_align2*)p}; }
+  static __device__ __forceinline__ Raw stream(const type* p) { return {__builtin_nontemporal_load((const u32x4_align2*)p)}; }
   static __device__ __forceinline__ void store(type* p, const Raw& r) { *(u32x4_align2*)p = r.a; }
+  static __device__ __forceinline__ void stream_out(type* p, const Raw& r) {
+    asm volatile("");
+    __builtin_nontemporal_store(r.a, (u32x4_align2*)p);
+    asm volatile("");
+  }
   static __device__ __forceinline__ Raw zero() { return {u32x4{0, 0, 0, 0}}; }
   static __device__ __forceinline__ void unpack(const Raw& r, float (&f)[8]) {
 #pragma unroll
@@ -105,7 +125,13 @@ struct Elem<OPTIMI_F16> {
   static __device__ __forceinline__ float get(type v) { return (float)v; }
   static __device__ __forceinline__ type put(float v) { return (type)v; }
   static __device__ __forceinline__ Raw load(const type* p) { return {*(const u32x4_align2*)p}; }
+  static __device__ __forceinline__ Raw stream(const type* p) { return {__builtin_nontemporal_load((const u32x4_align2*)p)}; }
   static __device__ __forceinline__ void store(type* p, const Raw& r) { *(u32x4_align2*)p = r.a; }
+  static __device__ __forceinline__ void stream_out(type* p, const Raw& r) {
+    asm volatile("");
+    __builtin_nontemporal_store(r.a, (u32x4_align2*)p);
+    asm volatile("");
+  }
   static __device__ __forceinline__ Raw zero() { return {u32x4{0, 0, 0, 0}}; }
   static __device__ __forceinline__ void unpack(const Raw& r, float (&f)[8]) {
 #pragma unroll
@@ -137,9 +163,10 @@ __device__ __forceinline__ typename Elem<DT>::Raw load_some(const typename Elem<
   return Elem<DT>::pack(f);
 }
 template <int DT>
-__device__ __forceinline__ void store_some(typename Elem<DT>::type* p, const float (&f)[8], int64_t n) {
+__device__ __forceinline__ void store_some(typename Elem<DT>::type* p, const float (&f)[8], int64_t n, bool stream = false) {
   if (n >= 8) {
-    Elem<DT>::store(p, Elem<DT>::pack(f));
+    if (stream) Elem<DT>::stream_out(p, Elem<DT>::pack(f));
+    else Elem<DT>::store(p, Elem<DT>::pack(f));
     return;
   }
 #pragma unroll

@@ -357,7 +357,7 @@ struct MatmulTile {
             float f[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) f[e] = fmaf((float)(int32_t)v[e] * sa, sb[e], bias[e]);
-            store_some<DT>((T*)p.out + m * p.n + n, f, some);
+            store_some<DT>((T*)p.out + m * p.n + n, f, some, whole_lines(p.n, sizeof(T)));
           }
         }
       }
@@ -728,7 +728,7 @@ __device__ __forceinline__ void store_sums(const WeightGradArgs& p, const f32x4 
       const float(&f)[8] = reinterpret_cast<const float(&)[8]>(v);
       if (n < p.outs && some > 0) {
         if (p.splits > 1) store_some<OPTIMI_F32>(p.partial + ((int64_t)split * p.outs + n) * p.cols + c, f, some);
-        else store_some<DT>((T*)p.out + n * p.cols + c, f, some);
+        else store_some<DT>((T*)p.out + n * p.cols + c, f, some, whole_lines(p.cols, sizeof(T)));
       }
     }
     __builtin_amdgcn_wave_barrier();

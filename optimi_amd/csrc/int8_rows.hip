@@ -49,9 +49,16 @@ __device__ __forceinline__ typename Elem<DT>::Raw load8(const typename Elem<DT>:
   if (TINY && cols < 8) return load_some<DT>(row, cols);
   return Elem<DT>::load(row + place8(c, cols));
 }
+// The same for what is read once.
 template <int DT, bool TINY>
-__device__ __forceinline__ void store8(typename Elem<DT>::type* row, int c, int cols, const float (&f)[8]) {
+__device__ __forceinline__ typename Elem<DT>::Raw stream8(const typename Elem<DT>::type* row, int c, int cols) {
+  if (TINY && cols < 8) return load_some<DT>(row, cols);
+  return Elem<DT>::stream(row + place8(c, cols));
+}
+template <int DT, bool TINY>
+__device__ __forceinline__ void store8(typename Elem<DT>::type* row, int c, int cols, const float (&f)[8], bool stream = false) {
   if (TINY && cols < 8) store_some<DT>(row, f, cols);
+  else if (stream) Elem<DT>::stream_out(row + place8(c, cols), Elem<DT>::pack(f));
   else Elem<DT>::store(row + place8(c, cols), Elem<DT>::pack(f));
 }
 template <bool TINY>
@@ -85,7 +92,7 @@ __global__ void __launch_bounds__(kLanes<TEAM>) quantize_kernel(const typename E
     for (int v = 0; v < VPT; ++v) {
       const int c = (v * TEAM + at.lane) * 8;
       raw[v] = E::zero();
-      if (c < cols) raw[v] = load8<DT, kTiny>(in, c, cols);
+      if (c < cols) raw[v] = stream8<DT, kTiny>(in, c, cols);
     }
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
@@ -145,14 +152,14 @@ __global__ void __launch_bounds__(kBlock) dequantize_kernel(const int8_t* __rest
     for (int c = lane * 8; c < cols; c += team * 8) {
       float f[8];
       if (cols >= 8) {
-        const u32x2 q = *(const u32x2_align1*)(from + place8(c, cols));
+        const u32x2 q = __builtin_nontemporal_load((const u32x2_align1*)(from + place8(c, cols)));
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] = (float)(int8_t)(q[i / 4] >> (8 * (i % 4))) * s;
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) f[i] = (float)from[i < cols ? i : 0] * s;
       }
-      store8<DT, true>(out + row * cols, c, cols, f);
+      store8<DT, true>(out + row * cols, c, cols, f, whole_lines(cols, sizeof(typename Elem<DT>::type)));
     }
   }
 }
@@ -210,14 +217,14 @@ __global__ void __launch_bounds__(kLanes<TEAM>) norm_kernel(NormArgs a) {
     for (int v = 0; v < VPT; ++v) {
       const int c = (v * TEAM + at.lane) * 8;
       raw[v] = E::zero();
-      if (c < cols) raw[v] = load8<DT, kTiny>((const T*)a.x + row * cols, c, cols);
+      if (c < cols) raw[v] = stream8<DT, kTiny>((const T*)a.x + row * cols, c, cols);
     }
     if (a.residual) {
 #pragma unroll
       for (int v = 0; v < VPT; ++v) {
         const int c = (v * TEAM + at.lane) * 8;
         if (c < cols) {
-          raw[v] = add_rows<DT>(raw[v], load8<DT, kTiny>((const T*)a.residual + row * cols, c, cols));
+          raw[v] = add_rows<DT>(raw[v], stream8<DT, kTiny>((const T*)a.residual + row * cols, c, cols));
           float f[8];
           E::unpack(raw[v], f);
           store8<DT, kTiny>((T*)a.h + row * cols, c, cols, f);
@@ -354,9 +361,9 @@ __global__ void __launch_bounds__(kLanes<TEAM>) norm_backward_kernel(NormBackwar
       const int c = (v * TEAM + at.lane) * 8;
       g[v] = h[v] = more[v] = E::zero();
       if (c < cols) {
-        g[v] = load8<DT, kTiny>((const T*)a.grad + row * cols, c, cols);
-        h[v] = load8<DT, kTiny>((const T*)a.h + row * cols, c, cols);
-        if (a.grad_h) more[v] = load8<DT, kTiny>((const T*)a.grad_h + row * cols, c, cols);
+        g[v] = stream8<DT, kTiny>((const T*)a.grad + row * cols, c, cols);
+        h[v] = stream8<DT, kTiny>((const T*)a.h + row * cols, c, cols);
+        if (a.grad_h) more[v] = stream8<DT, kTiny>((const T*)a.grad_h + row * cols, c, cols);
       }
     }
     float dot = 0.0f;
