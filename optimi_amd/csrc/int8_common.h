@@ -285,6 +285,7 @@ inline int check_shape(int64_t rows, int64_t cols) {
 }
 
 // Column sums of a [rows, cols] matrix in its own type (int8_rows.hip); the workspace holds fp32 partial rows.
+int finish_columns(const float* partial, int64_t parts, int64_t cols, int dtype, void* out, hipStream_t stream);  // the partial rows alone
 int64_t column_sum_workspace(int64_t rows, int64_t cols);
 int column_sum(const void* x, int64_t rows, int64_t cols, int dtype, void* out, void* workspace, hipStream_t stream);
 

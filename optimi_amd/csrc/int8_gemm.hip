@@ -632,6 +632,8 @@ struct WeightGradArgs {
   float* partial;  // [splits][outs][cols] where the sum is split
   int splits;
   int steps_per_split;
+  void* bias;           // sums of the gradient over rows, or NULL: by the workgroups of the first columns' tiles, which
+  float* bias_partial;  // have all gradients in their hands anyway; [splits][outs] where the sum is split
 };
 
 template <int DT>
@@ -858,6 +860,18 @@ __global__ void __launch_bounds__(512) weight_grad_kernel(WeightGradArgs p) {
       }
     }
   };
+  const bool with_bias = p.bias && tile.col == 0;
+  float bias[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  auto add_bias = [&](const Part& v) OPTIMI_INLINE {
+    if (!with_bias) return;
+#pragma unroll
+    for (int i = 0; i < kGrad; ++i) {
+      float f[8];
+      E::unpack(v.g[i], f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) bias[e] += f[e];
+    }
+  };
   auto multiply = [&](auto which, auto more, const Part& v) OPTIMI_INLINE {
     const short *g = which.value ? g1 : g0, *q = which.value ? q1 : q0;
     short *next_g = which.value ? g0 : g1, *next_q = which.value ? q0 : q1;
@@ -883,7 +897,10 @@ __global__ void __launch_bounds__(512) weight_grad_kernel(WeightGradArgs p) {
       if (more.value) turn(at, v, t, next_g, next_q);
       __builtin_amdgcn_sched_barrier(0);
     }
-    if (more.value) turn_special(v, t, next_g);
+    if (more.value) {
+      turn_special(v, t, next_g);
+      add_bias(v);
+    }
   };
   run_loaded(begin, end, part, load,
              [&](auto which, const Part& v) OPTIMI_INLINE {
@@ -891,8 +908,25 @@ __global__ void __launch_bounds__(512) weight_grad_kernel(WeightGradArgs p) {
 #pragma unroll
                for (int at = 0; at < kGroups; ++at) turn(at, v, t, which.value ? g1 : g0, which.value ? q1 : q0);
                turn_special(v, t, which.value ? g1 : g0);
+               add_bias(v);
              },
              multiply);
+  if (with_bias) {  // 32 lanes have sums of the same columns
+    float* sums = (float*)g0;
+    static_assert(32 * kTile * 4 <= kPlane * 2, "the sums fit a tile");
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sums[g_row * kTile + g_col + e] = bias[e];
+    __syncthreads();
+    const int64_t n = n0 + threadIdx.x;
+    if (threadIdx.x < kTile && n < p.outs) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int r = 0; r < 32; ++r) sum += sums[r * kTile + threadIdx.x];
+      if (p.splits > 1) p.bias_partial[split * p.outs + n] = sum;
+      else ((T*)p.bias)[n] = E::put(sum);
+    }
+  }
 
   using O = OutBlock<16, 32>;
   static_assert(kWaves / 2 * O::kBytes <= kPlane * 2, "half of the waves' blocks fit a tile");
@@ -1200,18 +1234,22 @@ MatmulPlan matmul_plan(int64_t m, int64_t n, int64_t k) {
 }
 
 struct WeightGradPlan {
-  bool pad;  // a padded copy of the gradient comes first
+  bool pad;       // a padded copy of the gradient comes first
+  bool bias_own;  // the bias gradient takes launches of its own
   Cut cut;
   int64_t pad_bytes, partial_bytes, bias_bytes;
 };
 WeightGradPlan weight_grad_plan(int64_t rows, int64_t outs, int64_t cols, int dtype, bool with_bias) {
   WeightGradPlan plan{};
-  plan.bias_bytes = with_bias ? padded(column_sum_workspace(rows, outs)) : 0;
-  if (cols == 0) return plan;
-  plan.cut = weight_grad_cut(rows, outs, cols, dtype);
-  plan.pad = plan.cut.tile == 256 && outs % 8 != 0;
-  plan.pad_bytes = plan.pad ? rows * padded(outs * 2) : 0;
-  plan.partial_bytes = plan.cut.splits > 1 ? padded(plan.cut.splits * outs * cols * 4) : 0;
+  if (cols > 0) {
+    plan.cut = weight_grad_cut(rows, outs, cols, dtype);
+    plan.pad = plan.cut.tile == 256 && outs % 8 != 0;
+    plan.pad_bytes = plan.pad ? rows * padded(outs * 2) : 0;
+    plan.partial_bytes = plan.cut.splits > 1 ? padded(plan.cut.splits * outs * cols * 4) : 0;
+  }
+  plan.bias_own = with_bias && (cols == 0 || plan.cut.tile == 256);
+  if (plan.bias_own) plan.bias_bytes = padded(column_sum_workspace(rows, outs));
+  else if (with_bias && plan.cut.splits > 1) plan.bias_bytes = padded(plan.cut.splits * outs * 4);
   return plan;
 }
 
@@ -1332,12 +1370,14 @@ int optimi_hip_int8_weight_grad(const void* grad, const int8_t* values, const fl
   if (plan.pad_bytes + plan.partial_bytes + plan.bias_bytes > 0 && !workspace) return OPTIMI_ERR_NULL;
   hipStream_t stream = (hipStream_t)stream_;
   int8_t* work = (int8_t*)workspace;
-  if (bias_grad) {
-    if (int rc = column_sum(grad, rows, outs, dtype, bias_grad, work + plan.pad_bytes + plan.partial_bytes, stream)) return rc;
+  float* bias_work = (float*)(work + plan.pad_bytes + plan.partial_bytes);
+  if (plan.bias_own) {
+    if (int rc = column_sum(grad, rows, outs, dtype, bias_grad, bias_work, stream)) return rc;
   }
   if (cols == 0) return 0;
   Cut c = plan.cut;
-  WeightGradArgs args{grad, outs, values, scales, rows, outs, cols, weight_grad, (float*)(work + plan.pad_bytes), c.splits, c.steps_per_split};
+  WeightGradArgs args{grad, outs, values, scales, rows, outs, cols, weight_grad, (float*)(work + plan.pad_bytes), c.splits, c.steps_per_split,
+                      plan.bias_own ? nullptr : bias_grad, bias_work};
   if (plan.pad) {
     if (int rc = pad_rows(grad, rows, nullptr, 0, outs * 2, work, stream)) return rc;
     args.grad = work;
@@ -1364,6 +1404,7 @@ int optimi_hip_int8_weight_grad(const void* grad, const int8_t* values, const fl
       const int64_t blocks = (outs * cols + 1023) / 1024;
       weight_grad_finish_kernel<DT><<<dim3((unsigned)(blocks < 4096 ? blocks : 4096)), dim3(256), 0, stream>>>(args);
       OPTIMI_INT8_TRY(hipGetLastError());
+      if (args.bias) return finish_columns(bias_work, c.splits, outs, dtype, bias_grad, stream);
     }
     return 0;
   });

@@ -540,6 +540,10 @@ inline int64_t norm_partials(int64_t rows, int64_t cols) {
   return partial_blocks(rows, cols) * rows_per_block(cols);
 }
 
+}  // namespace
+
+namespace optimi_int8 {
+
 int finish_columns(const float* partial, int64_t parts, int64_t cols, int dtype, void* out, hipStream_t stream) {
   if (cols == 0) return 0;
   return by_dtype(dtype, [&](auto dt) {
@@ -549,10 +553,6 @@ int finish_columns(const float* partial, int64_t parts, int64_t cols, int dtype,
     return 0;
   });
 }
-
-}  // namespace
-
-namespace optimi_int8 {
 
 // Column sums of a [rows, cols] matrix, for bias gradients: see int8_gemm.hip.
 int64_t column_sum_workspace(int64_t rows, int64_t cols) { return (rows < 128 ? rows : 128) * cols * 4; }

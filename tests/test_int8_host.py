@@ -54,7 +54,7 @@ def test_products_check_their_arguments():
     assert wg(P, P, P, 4, -4, 8, cabi.F32, P, None, P, None) == -2
     assert wg(None, P, P, 4, 4, 8, cabi.F32, P, None, P, None) == -1
     assert wg(P, P, P, 4, 4, 8, cabi.F32, None, None, P, None) == -1
-    assert wg(P, P, P, 4, 4, 8, cabi.F32, P, P, None, None) == -1  # a bias gradient needs the workspace
+    assert wg(P, P, P, 4096, 512, 512, cabi.F32, P, P, None, None) == -1  # a sum that is split needs the workspace
     assert wg(P, P, P, 4, 4, 8, cabi.F32, ODD, None, P, None) == -4
     assert wg(None, None, None, 4, 0, 8, cabi.F32, None, None, None, None) == 0
     assert L.optimi_hip_int8_weight_grad_workspace(4, 4, 8, 5, 0) == -3
