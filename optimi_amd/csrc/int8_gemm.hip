@@ -1304,6 +1304,7 @@ int optimi_hip_int8_matmul(const int8_t* a, const float* a_scales, const int8_t*
   if (plan.pad_bytes + plan.partial_bytes > 0 && !workspace) return OPTIMI_ERR_NULL;
   hipStream_t stream = (hipStream_t)stream_;
   MatmulArgs args{a, a_scales, b, b_scales, bias, m, n, k, out, nullptr, 1, 0};
+  if (plan.vec && (n + 15) / 16 > 2 * kMostTiles) return OPTIMI_ERR_SIZE;
   if (plan.vec) return by_dtype(dtype, [&](auto dt) { return launch_vec<decltype(dt)::value>(args, stream); });
 
   Cut c = plan.cut;

@@ -104,9 +104,19 @@ class _Int8Linear(torch.autograd.Function):
         return dx, dw if ctx.needs_input_grad[1] else None, db
 
 
+def _autocast(*tensors):
+    """Under ``torch.autocast`` a linear layer runs in the autocast dtype, as ``nn.Linear`` does."""
+    if not torch.is_autocast_enabled("cuda"):
+        return tensors
+    dtype = torch.get_autocast_dtype("cuda")
+    return tuple(None if t is None else t.to(dtype) for t in tensors)
+
+
 def int8_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None) -> Tensor:
     """``x @ weight.T + bias`` with x and weight quantized to int8 by rows, differentiable.  The backward pass
-    keeps x in 8 bits; quantization passes gradients straight through."""
+    keeps x in 8 bits; quantization passes gradients straight through.  Input, weight and bias are of one dtype;
+    under ``torch.autocast`` they are cast to its dtype first."""
+    x, weight, bias = _autocast(x, weight, bias)
     _check_linear(x, weight, bias)
     return _Int8Linear.apply(x, weight, bias)
 
@@ -150,11 +160,14 @@ def add_rms_norm_int8_linear(x: Tensor, norm_weight: Tensor, weights: Sequence[T
                              residual: Tensor | None = None, eps: float = 1e-6) -> tuple[tuple[Tensor, ...], Tensor]:
     """``(outputs, h)``: ``h = x + residual`` (``x`` itself without a residual) and, for every weight, the int8 linear
     layer of ``rms_norm(h) * norm_weight``, differentiable.  The normed activation exists as int8 only: one checkpoint
-    that all the layers (query, key and value, or gate and up) multiply and all their weight gradients read."""
+    that all the layers (query, key and value, or gate and up) multiply and all their weight gradients read.  ``norm_weight`` has
+    x's dtype or float32; ``torch.autocast`` casts as in ``int8_linear`` (and ``h`` is of the autocast dtype then)."""
     weights = tuple(weights)
     biases = (None,) * len(weights) if biases is None else tuple(biases)
     if not weights or len(biases) != len(weights):
         raise ValueError(f"optimi_amd: got {len(weights)} weights and {len(biases)} biases")
+    x, residual = _autocast(x, residual)
+    weights, biases = _autocast(*weights), _autocast(*biases)
     for w, b in zip(weights, biases):
         _check_linear(x, w, b)
     outs = _AddRmsNormInt8Linear.apply(x, residual, norm_weight, eps, *weights, *biases)

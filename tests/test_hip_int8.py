@@ -87,7 +87,7 @@ def test_quantize_at_the_ends_of_the_range(hip_device, dtype):
 
 SHAPES = [(1, 1, 1), (1, 16, 64), (1, 4096, 1024), (1, 77, 333), (2, 100, 129), (5, 33, 17), (15, 64, 256), (16, 65, 255), (17, 64, 256), (31, 130, 1000),
           (33, 200, 4096), (63, 255, 640), (64, 256, 128), (65, 257, 129), (127, 128, 127), (128, 512, 384), (129, 300, 70), (255, 256, 2048), (256, 256, 256),
-          (257, 513, 1025), (300, 1000, 272), (512, 768, 1040), (700, 40, 3000), (1030, 770, 528), (40, 700, 16), (200, 300, 0), (0, 5, 7), (5, 0, 7), (300, 300, 11008)]
+          (257, 513, 1025), (300, 1000, 272), (512, 768, 1040), (700, 40, 3000), (1030, 770, 528), (40, 700, 16), (200, 300, 0), (3, 300, 0), (0, 5, 7), (5, 0, 7), (300, 300, 11008)]
 
 
 def int8_inputs(m, n, k, seed, pow2=True):
@@ -408,6 +408,36 @@ def test_linear_and_its_gradients(hip_device, shape, dtype, bias):
     R.close(leaves[0].grad.view(-1, k), dx, slack + R.half(dtype) * (dx.abs() + slack) + 1.01 * R.least(dtype), "dx")
 
 
+def test_linear_of_a_single_vector_and_of_no_rows(hip_device):
+    w, b = rand((40, 24), torch.float32, 1).to(hip_device).requires_grad_(), rand((40,), torch.float32, 2).to(hip_device).requires_grad_()
+    x = rand((1, 24), torch.float32, 3).to(hip_device)
+    flat = x[0].clone().requires_grad_()
+    y = optimi.int8_linear(flat, w, b)
+    assert y.shape == (40,) and torch.equal(y, optimi.int8_linear(x, w, b)[0])
+    y.sum().backward()
+    assert flat.grad.shape == (24,) and w.grad.shape == (40, 24) and torch.equal(b.grad, torch.ones_like(b))
+    (y,), h = optimi.add_rms_norm_int8_linear(flat, torch.ones(24, device=hip_device), [w], residual=x[0])
+    assert y.shape == (40,) and h.shape == (24,)
+    (y.sum() + h.sum()).backward()
+    w.grad = b.grad = None
+    none = torch.zeros(0, 24, device=hip_device, requires_grad=True)
+    optimi.int8_linear(none, w, b).sum().backward()
+    assert none.grad.shape == (0, 24) and not w.grad.any() and not b.grad.any()
+
+
+def test_linear_under_autocast(hip_device):
+    layer = optimi.Int8Linear(64, 32).to(hip_device)
+    x = torch.randn(9, 64, device=hip_device, requires_grad=True)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = layer(x)
+        (z,), h = optimi.add_rms_norm_int8_linear(x, torch.ones(64, device=hip_device), [layer.weight], [layer.bias], residual=x)
+    assert y.dtype == z.dtype == h.dtype == torch.bfloat16
+    want = optimi.int8_linear(x.bfloat16(), layer.weight.bfloat16(), layer.bias.bfloat16())
+    assert torch.equal(y, want)
+    (y.float().sum() + z.float().sum() + h.float().sum()).backward()
+    assert x.grad.dtype == layer.weight.grad.dtype == layer.bias.grad.dtype == torch.float32
+
+
 def test_linear_keeps_only_what_it_needs(hip_device):
     x, w = torch.randn(64, 256, device=hip_device), torch.randn(128, 256, device=hip_device)
     y = optimi.int8_linear(x.clone().requires_grad_(), w)  # a frozen weight needs no checkpoint
@@ -673,6 +703,112 @@ def test_on_another_stream(hip_device):
     torch.cuda.synchronize()
     for got in outs:
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---------------------------------------------------------------------------------- the C boundary
+
+class Guarded:
+    """Device buffers with a margin of a known pattern on both sides."""
+
+    def __init__(self, device):
+        self.device, self.made = device, []
+
+    def __call__(self, like=None, shape=None, dtype=None, offset=0):
+        shape, dtype = (tuple(like.shape), like.dtype) if like is not None else (shape, dtype)
+        size = torch.empty((), dtype=dtype).element_size()
+        n = size
+        for d in shape:
+            n *= d
+        room = torch.full((n + 1024 + offset * size,), 0x5A, dtype=torch.uint8, device=self.device)
+        inner = room[512 + offset * size: 512 + offset * size + n]
+        view = inner.view(dtype).view(shape) if n else torch.empty(shape, dtype=dtype, device=self.device)
+        if like is not None:
+            view.copy_(like)
+        self.made.append((room, 512 + offset * size, n, like))
+        return view
+
+    def check(self):
+        for room, first, n, like in self.made:
+            assert bool((room[:first] == 0x5A).all()) and bool((room[first + n:] == 0x5A).all()), "wrote outside of a buffer"
+            if like is not None:
+                assert torch.equal(room[first:first + n].cpu(), like.contiguous().view(-1).view(torch.uint8)), "wrote an input"
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES, ids=R.IDS)
+@pytest.mark.parametrize("shape", [(1, 5, 3), (3, 40, 7), (9, 33, 17), (65, 100, 1000), (130, 257, 129), (70, 1001, 515), (2600, 2700, 131), (40, 20, 17001)],
+                         ids=lambda s: "x".join(map(str, s)))
+def test_nothing_outside_of_the_outputs_is_written(hip_device, shape, dtype):
+    """Every operator through the C ABI, into buffers one element off the grid with margins around them."""
+    from optimi_amd import cabi
+    L, code = cabi.lib(), {torch.float32: cabi.F32, torch.bfloat16: cabi.BF16, torch.float16: cabi.F16}[dtype]
+    m, n, k = shape
+    x, r, g, w, bias = rand((m, k), dtype, 1), rand((m, k), dtype, 2), rand((m, n), dtype, 3), rand((n, k), dtype, 4), rand((n,), dtype, 5)
+    nw = rand((k,), dtype, 6)
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def run(name, *args):
+        cabi.check(getattr(L, "optimi_hip_" + name)(*(a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args), stream), name)
+
+    def work(name, *args):
+        size = getattr(L, "optimi_hip_" + name + "_workspace")(*args)
+        assert size >= 0
+        return buf(shape=(size,), dtype=torch.uint8) if size else None
+
+    for offset in (0, 1):
+        buf = Guarded(hip_device)
+        out = lambda *s, t=dtype: buf(shape=s, dtype=t, offset=offset)  # noqa: E731
+        dx, dr, dg, dw, db, dn = (buf(t, offset=offset) for t in (x, r, g, w, bias, nw))
+        q, s, wq, ws = out(m, k, t=torch.int8), out(m, t=torch.float32), out(n, k, t=torch.int8), out(n, t=torch.float32)
+        run("int8_quantize", dx, m, k, code, q, s)
+        run("int8_quantize", dw, n, k, code, wq, ws)
+        back = out(m, k)
+        run("int8_dequantize", q, s, m, k, code, back)
+        y = out(m, n)
+        run("int8_matmul", q, s, wq, ws, db, m, n, k, code, y, work("int8_matmul", m, n, k))
+        gw, gb = out(n, k), out(n)
+        run("int8_weight_grad", dg, q, s, m, n, k, code, gw, gb, work("int8_weight_grad", m, n, k, code, 1))
+        h, q2, s2, rstd = out(m, k), out(m, k, t=torch.int8), out(m, t=torch.float32), out(m, t=torch.float32)
+        run("add_rms_norm_int8", dx, dr, dn, m, k, code, code, 1e-6, h, q2, s2, rstd)
+        gx, gn = out(m, k), out(k)
+        run("add_rms_norm_int8_backward", back, dr, h, rstd, dn, m, k, code, code, gx, gn, work("add_rms_norm_int8_backward", m, k))
+        torch.cuda.synchronize()
+        buf.check()
+        wq64, ws64 = R.quantize(w)
+        x64, s64 = R.quantize(x)
+        assert torch.equal(q.cpu().double(), x64) and torch.equal(s.cpu().double(), s64)
+        R.close(y, *R.matmul(x64, s64, wq64, ws64, bias, dtype), "y")
+        R.close(gw, *R.weight_grad(g, x64, s64, dtype), "gw")
+        R.close(gb, *R.column_sum(g, dtype), "gb")
+        assert torch.equal(h.cpu(), (x.double() + r.double()).to(dtype))
+
+
+def test_offsets_beyond_32_bits(hip_device):
+    """Rows behind the 2^32nd element give what they give alone."""
+    rows, cols, outs, last = (1 << 20) + 100, 4100, 24, 300
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB of device memory")
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device=hip_device)
+    tail = rand((last, cols), torch.bfloat16, 1).to(hip_device)
+    x[-last:] = tail
+    values, scales = optimi.int8_quantize(x)
+    q, s = optimi.int8_quantize(tail)
+    assert torch.equal(values[-last:], q) and torch.equal(scales[-last:], s) and not values[:-last].any()
+    assert torch.equal(optimi.int8_dequantize(values, scales)[-last:], optimi.int8_dequantize(q, s))
+    w, ws = optimi.int8_quantize(rand((outs, cols), torch.bfloat16, 2).to(hip_device))
+    assert torch.equal(optimi.int8_matmul(values, scales, w, ws)[-last:], optimi.int8_matmul(q, s, w, ws))
+    g = torch.zeros(rows, outs, dtype=torch.bfloat16, device=hip_device)
+    g[-last:] = rand((last, outs), torch.bfloat16, 3, 1e-2).to(hip_device)
+    dw, db = optimi.int8_weight_grad(g, values, scales, bias=True)
+    want, allowed = R.weight_grad(g[-last:], q, s, torch.bfloat16)
+    R.close(dw, want.cpu(), allowed.cpu(), "weight gradient")
+    nw = torch.ones(cols, dtype=torch.bfloat16, device=hip_device)
+    del values
+    nv, ns, h, rstd = optimi.add_rms_norm_int8(x, nw, residual=x)
+    nv2, ns2, h2, rstd2 = optimi.add_rms_norm_int8(tail, nw, residual=tail)
+    assert torch.equal(nv[-last:], nv2) and torch.equal(ns[-last:], ns2) and torch.equal(h[-last:], h2) and torch.equal(rstd[-last:], rstd2)
+    del nv
+    dx, _ = optimi.add_rms_norm_int8_backward(x, h, rstd, nw)
+    assert torch.equal(dx[-last:], optimi.add_rms_norm_int8_backward(tail, h2, rstd2, nw)[0])
 
 
 # ---------------------------------------------------------------------------------- refusals
