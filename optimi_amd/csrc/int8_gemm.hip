@@ -1176,7 +1176,8 @@ inline int64_t tiles_of(int64_t rows, int64_t cols, int tile) { return ((rows + 
 // 2.05 per round of 256; 128 x 128 tiles 0.68, 0.82 up to one per CU, 1.2 per round of two per CU; 64 x 64 tiles 0.25 up to
 // one per CU, then 0.22 for each further one.  (2048 x 4096 x 4096: 52 us in tiles of 256, 41 in tiles of 128, 60 in
 // tiles of 64; 4096 x 4096 x 4096: 66, 77, 112; 512 x 4096 x 4096: 47, 24, 18.)  Few tiles with a long sum are split, one part
-// per idle CU, eight steps at least each: 100 x 100 x 16384 takes 23 us whole and 9.2 us in 16 parts.
+// per idle CU, eight steps at least each: 100 x 100 x 16384 takes 23 us whole and 9.2 us in 16 parts.  Below 40 steps the
+// second launch costs what the parts save: 64 x 4096 x 4096 takes 9.1 us whole, 10.9 us in four parts.
 Cut matmul_cut(int64_t m, int64_t n, int64_t k) {
   const int64_t steps = (k + kStep - 1) / kStep;
   const int64_t t256 = tiles_of(m, n, 256), t128 = tiles_of(m, n, 128), t64 = tiles_of(m, n, 64);
@@ -1187,7 +1188,7 @@ Cut matmul_cut(int64_t m, int64_t n, int64_t k) {
   c.tile = c256 <= c128 && c256 <= c64 ? 256 : c128 <= c64 ? 128 : 64;
   c.tiles = c.tile == 256 ? t256 : c.tile == 128 ? t128 : t64;
   int64_t parts = 1;
-  if (c.tile == 64 && c.tiles < kCus) parts = kCus / c.tiles < steps / 8 ? kCus / c.tiles : steps / 8;
+  if (c.tile == 64 && c.tiles < kCus && steps >= 40) parts = kCus / c.tiles < steps / 8 ? kCus / c.tiles : steps / 8;
   c.split(steps, parts < 16 ? parts : 16);
   return c;
 }
