@@ -1175,9 +1175,9 @@ inline int64_t tiles_of(int64_t rows, int64_t cols, int tile) { return ((rows + 
 // the whole machine, int8 operands that come from the caches: 256 x 256 tiles 1.55 where they leave half of the 256 CUs empty,
 // 2.05 per round of 256; 128 x 128 tiles 0.68, 0.82 up to one per CU, 1.2 per round of two per CU; 64 x 64 tiles 0.25 up to
 // one per CU, then 0.22 for each further one.  (2048 x 4096 x 4096: 52 us in tiles of 256, 41 in tiles of 128, 60 in
-// tiles of 64; 4096 x 4096 x 4096: 66, 77, 112; 512 x 4096 x 4096: 47, 24, 18.)  Few tiles with a long sum are split, one part
-// per idle CU, eight steps at least each: 100 x 100 x 16384 takes 23 us whole and 9.2 us in 16 parts.  Below 40 steps the
-// second launch costs what the parts save: 64 x 4096 x 4096 takes 9.1 us whole, 10.9 us in four parts.
+// tiles of 64; 4096 x 4096 x 4096: 66, 77, 112; 512 x 4096 x 4096: 47, 24, 18.)  Few tiles with a long sum are split into parts
+// for the idle CUs where that saves more than the joining launch costs, 3.5 us and the partial sums' way to memory and back:
+// 100 x 100 x 16384 takes 23 us whole and 9.2 us in 16 parts, 64 x 4096 x 4096 9.1 us whole and 10.9 us in four.
 Cut matmul_cut(int64_t m, int64_t n, int64_t k) {
   const int64_t steps = (k + kStep - 1) / kStep;
   const int64_t t256 = tiles_of(m, n, 256), t128 = tiles_of(m, n, 128), t64 = tiles_of(m, n, 64);
@@ -1188,8 +1188,17 @@ Cut matmul_cut(int64_t m, int64_t n, int64_t k) {
   c.tile = c256 <= c128 && c256 <= c64 ? 256 : c128 <= c64 ? 128 : 64;
   c.tiles = c.tile == 256 ? t256 : c.tile == 128 ? t128 : t64;
   int64_t parts = 1;
-  if (c.tile == 64 && c.tiles < kCus && steps >= 40) parts = kCus / c.tiles < steps / 8 ? kCus / c.tiles : steps / 8;
-  c.split(steps, parts < 16 ? parts : 16);
+  if (c.tile == 64) {
+    double least = 0.25 * (double)steps;
+    for (int64_t s = 2; s <= 16 && s * c.tiles <= kCus && 4 * s <= steps; ++s) {
+      const double cost = 0.25 * (double)((steps + s - 1) / s) + 3.5 + (double)s * (double)m * (double)n * 8 / 3e6;
+      if (cost < least) {
+        least = cost;
+        parts = s;
+      }
+    }
+  }
+  c.split(steps, parts);
   return c;
 }
 // The same for weight gradients, in microseconds per step of 64 rows: 2.2 per round of 256 wide tiles; 0.8 for up to 256 tiles
@@ -1211,12 +1220,17 @@ Cut weight_grad_cut(int64_t rows, int64_t outs, int64_t cols, int dtype) {
   return c;
 }
 
-// Products of at most this many rows are read off the weight without tiles.
-constexpr int64_t kMostVec = 8;
+// Products of at most this many rows are read off the weight without tiles.  (1 x 11008 x 4096: 9.2 us, in tiles 14; 4 x 11008
+// x 4096: 9.3 us; 8 x 11008 x 4096: 15.5 us, in tiles 10.2.)
+constexpr int64_t kMostVec = 4;
 // Bytes that padded copies of the operands take, for rows that do not start on 16 bytes in tiles that are copied asynchronously.
 inline int64_t padded(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 
 // What a product of these sizes does: computed alike by the call and by its workspace function.
+//
+// Odd widths: large tiles are copied asynchronously and take padded copies of both operands.  Small ones can be loaded through registers,
+// at 0.45 us a step instead of 0.2; the copies cost a launch and 0.5 us per million bytes (measured: 42 x 216 x 3675 16.6 us through
+// registers, 13.3 us padded; 20 x 8000 x 8001 32 us, 38 us).
 struct MatmulPlan {
   bool vec;         // read off the weight
   bool pad;         // padded copies of both operands come first
@@ -1228,7 +1242,7 @@ MatmulPlan matmul_plan(int64_t m, int64_t n, int64_t k) {
   plan.vec = m <= kMostVec;
   if (plan.vec) return plan;
   plan.cut = matmul_cut(m, n, k);
-  plan.pad = k % 16 != 0 && plan.cut.tile > 64;
+  plan.pad = k % 16 != 0 && (plan.cut.tile > 64 || 0.25 * (double)((k + kStep - 1) / kStep) > 2.0 + 0.5e-6 * (double)((m + n) * k));
   plan.pad_bytes = plan.pad ? (m + n) * padded(k) : 0;
   plan.partial_bytes = plan.cut.splits > 1 ? plan.cut.splits * m * n * 4 : 0;
   return plan;
@@ -1266,8 +1280,7 @@ int launch_vec(const MatmulArgs& args, hipStream_t stream) {
   };
   if (args.m == 1) go(Pair<1>{});
   else if (args.m == 2) go(Pair<2>{});
-  else if (args.m <= 4) go(Pair<4>{});
-  else go(Pair<8>{});
+  else go(Pair<4>{});
   OPTIMI_INT8_TRY(hipGetLastError());
   return 0;
 }
