@@ -1,5 +1,6 @@
 /*
- * optimi_hip.h — C ABI of the MI355X (gfx950) fused optimizer-step library.
+ * optimi_hip.h — C ABI of the MI355X (gfx950) fused optimizer-step library, and of the
+ * int8 activation operators beside it (last section).
  *
  * The reference (warner-benjamin/optimi) has no FFI: its accelerated backend is a set
  * of Triton kernels launched from Python, one launch per tensor.  Each entry point
@@ -348,7 +349,8 @@ int64_t optimi_hip_launch_limit(int64_t workgroups);
  * type; values stay within +-63 under scales whose 64th multiple the type cannot hold.  A row
  * that holds an infinity or a NaN gets the scale NaN and zeros.  The products take any scales.
  *
- * All matrices are contiguous, rows < 2^31, cols <= 2^28 (OPTIMI_ERR_SIZE beyond).  Buffers need
+ * All matrices are contiguous, rows < 2^31, cols <= 2^28 (outs and cols <= 2^24 for the weight
+ * gradient), and a product has at most 2^22 tiles of 64 x 64 outputs or larger (OPTIMI_ERR_SIZE beyond).  Buffers need
  * only be aligned to their element size.  Workspaces are the caller's: as many bytes of device memory
  * as the _workspace function of the same name and sizes says (it returns a negative status for
  * sizes that the call would refuse), aligned to 16 bytes, not shared by calls that may

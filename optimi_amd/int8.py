@@ -199,7 +199,8 @@ class _Int8Sequential(nn.Sequential):
         while i < len(modules):
             if i + 1 < len(modules) and _is_norm_of(modules[i], modules[i + 1]):
                 norm, layer = modules[i], modules[i + 1]
-                eps = torch.finfo(x.dtype).eps if norm.eps is None else norm.eps
+                # nn.RMSNorm without an eps adds that of the type it computes in
+                eps = torch.finfo(torch.float32).eps if norm.eps is None else norm.eps
                 (x,), _ = add_rms_norm_int8_linear(x, norm.weight, [layer.weight], [layer.bias], eps=eps)
                 i += 2
             else:

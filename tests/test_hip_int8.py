@@ -614,9 +614,13 @@ def test_the_norm_in_a_sequence_hands_over_int8(hip_device):
         model = nn.Sequential(nn.RMSNorm(80, eps=eps), nn.Linear(80, 48)).to(torch.bfloat16).to(hip_device)
         optimi.prepare_for_int8_linear(model)
         x = rand((9, 80), torch.bfloat16, 1, 0.05).to(hip_device)
-        e = torch.finfo(torch.bfloat16).eps if eps is None else eps
+        e = torch.finfo(torch.float32).eps if eps is None else eps
         (want,), _ = optimi.add_rms_norm_int8_linear(x, model[0].weight, [model[1].weight], [model[1].bias], eps=e)
         assert torch.equal(model(x), want)
+        # the same eps as the module's own: its result, rounded to bf16, is half a step of either rounding away
+        values, scales, _, _ = optimi.add_rms_norm_int8(x, model[0].weight, eps=e)
+        plain = model[0](x).double()
+        assert bool(((values.double() * scales.double()[:, None] - plain).abs() <= scales.double()[:, None] / 2 + 2.1 * R.half(torch.bfloat16) * plain.abs()).all())
 
 
 # ---------------------------------------------------------------------------------- graphs, streams
