@@ -2,6 +2,7 @@
 // assume, makes them contiguous, allocates outputs and workspaces from PyTorch's allocator on the calling thread's
 // current stream, and raises RuntimeError when the library returns a non-zero status.
 
+#include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <torch/extension.h>
@@ -52,20 +53,27 @@ at::DimVector with_cols(const Tensor& t, int64_t cols) {
   return sizes;
 }
 
+// The calls are short, and on small inputs the host's part of them is what counts: tensors are made by the allocator's own
+// function instead of through the dispatcher, and a contiguous one is taken as it is.
+Tensor make(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+Tensor dense(const Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
+
 // values [..., cols] with one scale per row
 Tensor check_pair(const Tensor& values, const Tensor& scales, const char* name) {
   TORCH_CHECK(values.scalar_type() == at::kChar, "optimi_amd: ", name, " must hold int8 values, got ", values.scalar_type());
   TORCH_CHECK(scales.scalar_type() == at::kFloat, "optimi_amd: the scales of ", name, " must be float32, got ", scales.scalar_type());
   TORCH_CHECK(values.dim() >= 1 && scales.sizes() == values.sizes().slice(0, values.dim() - 1), "optimi_amd: ", name, " of size ", values.sizes(),
               " needs scales of size ", values.sizes().slice(0, values.dim() - 1), ", got ", scales.sizes());
-  return scales.contiguous();
+  return dense(scales);
 }
 
 hipStream_t current_stream() { return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA().stream(); }
 
 Tensor workspace(int64_t bytes, const Tensor& like, const char* what) {
   if (bytes < 0) check_status((int)bytes, what);
-  return bytes ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
+  return bytes ? make({bytes}, at::kByte, like) : Tensor();
 }
 void* pointer(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
@@ -74,9 +82,9 @@ std::tuple<Tensor, Tensor> int8_quantize(const Tensor& x_) {
   const int dtype = dtype_code(x_.scalar_type(), "the activation");
   const Rows r = rows_of(x_, "the activation");
   c10::hip::HIPGuardMasqueradingAsCUDA guard(x_.device());
-  const Tensor x = x_.contiguous();
-  Tensor values = at::empty(x.sizes(), x.options().dtype(at::kChar));
-  Tensor scales = at::empty(leading(x), x.options().dtype(at::kFloat));
+  const Tensor x = dense(x_);
+  Tensor values = make(x.sizes(), at::kChar, x);
+  Tensor scales = make(leading(x), at::kFloat, x);
   check_status(optimi_hip_int8_quantize(x.data_ptr(), r.rows, r.cols, dtype, (int8_t*)values.data_ptr(), (float*)scales.data_ptr(), current_stream()),
                "optimi_hip_int8_quantize");
   return {values, scales};
@@ -89,8 +97,8 @@ Tensor int8_dequantize(const Tensor& values_, const Tensor& scales_, at::ScalarT
   c10::hip::HIPGuardMasqueradingAsCUDA guard(values_.device());
   const Tensor scales = check_pair(values_, scales_, "values");
   const Rows r = rows_of(values_, "values");
-  const Tensor values = values_.contiguous();
-  Tensor out = at::empty(values.sizes(), values.options().dtype(type));
+  const Tensor values = dense(values_);
+  Tensor out = make(values.sizes(), type, values);
   check_status(optimi_hip_int8_dequantize((const int8_t*)values.data_ptr(), (const float*)scales.data_ptr(), r.rows, r.cols, dtype, out.data_ptr(),
                                           current_stream()),
                "optimi_hip_int8_dequantize");
@@ -115,10 +123,10 @@ Tensor int8_matmul(const Tensor& a_, const Tensor& a_scales_, const Tensor& b_, 
     check_device(a_, *bias_, "the bias");
     TORCH_CHECK(bias_->scalar_type() == type, "optimi_amd: the bias has dtype ", bias_->scalar_type(), ", the result ", type);
     TORCH_CHECK(bias_->dim() == 1 && bias_->size(0) == n, "optimi_amd: the bias must have ", n, " elements, got size ", bias_->sizes());
-    bias = bias_->contiguous();
+    bias = dense(*bias_);
   }
-  const Tensor a = a_.contiguous(), b = b_.contiguous();
-  Tensor out = at::empty(with_cols(a, n), a.options().dtype(type));
+  const Tensor a = dense(a_), b = dense(b_);
+  Tensor out = make(with_cols(a, n), type, a);
   const Tensor work = workspace(optimi_hip_int8_matmul_workspace(r.rows, n, r.cols), a, "optimi_hip_int8_matmul");
   check_status(optimi_hip_int8_matmul((const int8_t*)a.data_ptr(), (const float*)a_scales.data_ptr(), (const int8_t*)b.data_ptr(),
                                       (const float*)b_scales.data_ptr(), pointer(bias), r.rows, n, r.cols, dtype, out.data_ptr(), pointer(work),
@@ -137,10 +145,10 @@ std::tuple<Tensor, std::optional<Tensor>> int8_weight_grad(const Tensor& grad_, 
   const Rows g = rows_of(grad_, "the gradient"), v = rows_of(values_, "the checkpoint");
   TORCH_CHECK(leading(grad_) == leading(values_), "optimi_amd: the gradient of size ", grad_.sizes(), " and the checkpoint of size ", values_.sizes(),
               " have different rows");
-  const Tensor grad = grad_.contiguous(), values = values_.contiguous();
-  Tensor dw = at::empty({g.cols, v.cols}, grad.options());
+  const Tensor grad = dense(grad_), values = dense(values_);
+  Tensor dw = make({g.cols, v.cols}, grad.scalar_type(), grad);
   std::optional<Tensor> db;
-  if (with_bias) db = at::empty({g.cols}, grad.options());
+  if (with_bias) db = make({g.cols}, grad.scalar_type(), grad);
   const Tensor work = workspace(optimi_hip_int8_weight_grad_workspace(g.rows, g.cols, v.cols, dtype, with_bias), grad, "optimi_hip_int8_weight_grad");
   check_status(optimi_hip_int8_weight_grad(grad.data_ptr(), (const int8_t*)values.data_ptr(), (const float*)scales.data_ptr(), g.rows, g.cols, v.cols,
                                            dtype, dw.data_ptr(), db ? db->data_ptr() : nullptr, pointer(work), current_stream()),
@@ -172,12 +180,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> add_rms_norm_int8(const Tensor& x_, c
   c10::hip::HIPGuardMasqueradingAsCUDA guard(x_.device());
   if (residual_.has_value()) {
     check_twin(x_, *residual_, "the residual");
-    residual = residual_->contiguous();
+    residual = dense(*residual_);
   }
-  const Tensor x = x_.contiguous(), weight = weight_.contiguous();
-  Tensor values = at::empty(x.sizes(), x.options().dtype(at::kChar));
-  Tensor scales = at::empty(leading(x), x.options().dtype(at::kFloat)), rstd = at::empty_like(scales);
-  Tensor h = residual.defined() ? at::empty(x.sizes(), x.options()) : Tensor();
+  const Tensor x = dense(x_), weight = dense(weight_);
+  Tensor values = make(x.sizes(), at::kChar, x);
+  Tensor scales = make(leading(x), at::kFloat, x), rstd = make(leading(x), at::kFloat, x);
+  Tensor h = residual.defined() ? make(x.sizes(), x.scalar_type(), x) : Tensor();
   check_status(optimi_hip_add_rms_norm_int8(x.data_ptr(), pointer(residual), weight.data_ptr(), r.rows, r.cols, dtype, weight_dtype, eps, pointer(h),
                                             (int8_t*)values.data_ptr(), (float*)scales.data_ptr(), (float*)rstd.data_ptr(), current_stream()),
                "optimi_hip_add_rms_norm_int8");
@@ -198,10 +206,10 @@ std::tuple<Tensor, Tensor> add_rms_norm_int8_backward(const Tensor& grad_, const
   Tensor grad_h;
   if (grad_h_.has_value()) {
     check_twin(grad_, *grad_h_, "the gradient of h");
-    grad_h = grad_h_->contiguous();
+    grad_h = dense(*grad_h_);
   }
-  const Tensor grad = grad_.contiguous(), h = h_.contiguous(), rstd = rstd_.contiguous(), weight = weight_.contiguous();
-  Tensor dx = at::empty(grad.sizes(), grad.options()), dweight = at::empty({r.cols}, weight.options());
+  const Tensor grad = dense(grad_), h = dense(h_), rstd = dense(rstd_), weight = dense(weight_);
+  Tensor dx = make(grad.sizes(), grad.scalar_type(), grad), dweight = make({r.cols}, weight.scalar_type(), weight);
   const Tensor work = workspace(optimi_hip_add_rms_norm_int8_backward_workspace(r.rows, r.cols), grad, "optimi_hip_add_rms_norm_int8_backward");
   check_status(optimi_hip_add_rms_norm_int8_backward(grad.data_ptr(), pointer(grad_h), h.data_ptr(), (const float*)rstd.data_ptr(), weight.data_ptr(),
                                                      r.rows, r.cols, dtype, weight_dtype, dx.data_ptr(), dweight.data_ptr(), pointer(work),

@@ -16,6 +16,7 @@ stream are the caller's to synchronize, as everywhere in PyTorch.
 
 from __future__ import annotations
 
+import math
 import warnings
 from typing import Iterable, Sequence
 
@@ -85,6 +86,14 @@ def _product(values, scales, weight, bias, dtype):
     return int8_matmul(values, scales, weight_values, weight_scales, bias, dtype)
 
 
+def _times_weight(grad: Tensor, weight: Tensor, plus: Tensor | None = None) -> Tensor:
+    """``grad @ weight (+ plus)`` as one product of two matrices, whatever grad's dimensions and strides."""
+    shape, (n, k) = grad.shape[:-1], weight.shape
+    grad = grad.reshape(math.prod(shape), n)
+    out = grad.mm(weight) if plus is None else torch.addmm(plus.view(grad.shape[0], k), grad, weight)
+    return out.view(*shape, k)
+
+
 class _Int8Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
@@ -97,7 +106,7 @@ class _Int8Linear(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad):
         weight, values, scales = ctx.saved_tensors
-        dx = grad.matmul(weight) if ctx.needs_input_grad[0] else None
+        dx = _times_weight(grad, weight) if ctx.needs_input_grad[0] else None
         dw = db = None
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
             dw, db = backend.ext().int8_weight_grad(grad, values, scales, ctx.needs_input_grad[2])
@@ -144,8 +153,7 @@ class _AddRmsNormInt8Linear(torch.autograd.Function):
             if grad is None:
                 continue
             if need_x or need_residual or need_norm:
-                grad2, dy2 = grad.reshape(-1, weight.shape[0]), None if dy is None else dy.reshape(-1, weight.shape[1])
-                dy = (grad2.mm(weight) if dy2 is None else torch.addmm(dy2, grad2, weight)).reshape(h.shape)
+                dy = _times_weight(grad, weight, plus=dy)
             need_w, need_b = ctx.needs_input_grad[4 + i], ctx.needs_input_grad[4 + n + i]
             if need_w or need_b:
                 dw, dbs[i] = backend.ext().int8_weight_grad(grad, values, scales, need_b)
