@@ -377,7 +377,8 @@ int optimi_hip_int8_matmul(const int8_t* a, const float* a_scales, const int8_t*
  * weight_grad[n][k] = sum_r grad[r][n] * scales[r] * values[r][k], and bias_grad[n] = sum_r grad[r][n] where bias_grad
  * is not NULL.  grad [rows, outs], values [rows, cols], weight_grad [outs, cols]; all but values and scales are of
  * `dtype`.  Products of bf16 and fp16 gradients are formed with values[r][k] * scales[r] rounded to that type (exact
- * for this library's scales), those of fp32 gradients without rounding; sums are fp32.  rows = 0 writes zeros. */
+ * for this library's scales), those of fp32 gradients without rounding, where grad * scale lies between
+ * 2^-110 and the largest float; sums are fp32.  rows = 0 writes zeros. */
 int64_t optimi_hip_int8_weight_grad_workspace(int64_t rows, int64_t outs, int64_t cols, int dtype, int with_bias);
 int optimi_hip_int8_weight_grad(const void* grad, const int8_t* values, const float* scales, int64_t rows, int64_t outs,
                                 int64_t cols, int dtype, void* weight_grad, void* bias_grad, void* workspace,

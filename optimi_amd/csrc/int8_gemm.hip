@@ -718,15 +718,12 @@ __device__ __forceinline__ s16x8 read_column(const short* tile, int offset, int 
   return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
-// Four values as 16-bit numbers: bytes as unsigned numbers are 128 too large, (u - 128) s has one rounding, and none
-// under a power of two.
+// Four values as 16-bit numbers; their products with the scale have no rounding under a power of two.
 template <int DT>
 __device__ __forceinline__ u32x2 widen(uint32_t word, float s) {
-  const uint32_t u = word ^ 0x80808080u;
-  const float minus = -128.0f * s;
   float f[4];
 #pragma unroll
-  for (int e = 0; e < 4; ++e) f[e] = fmaf((float)((u >> (8 * e)) & 0xffu), s, minus);
+  for (int e = 0; e < 4; ++e) f[e] = (float)(int8_t)(word >> (8 * e)) * s;
   return u32x2{Product<DT>::pair(f[0], f[1]), Product<DT>::pair(f[2], f[3])};
 }
 
@@ -959,11 +956,12 @@ __global__ void __launch_bounds__(512) weight_grad_kernel(WeightGradArgs p) {
 // rows a step, two pairs of tiles in LDS, eight wavefronts with 128 x 64 sums each.  Gradients go to LDS past the registers;
 // the values have to become 16-bit numbers on the way, and are loaded two steps ahead, so that the conversion of the next
 // step's values can be spread over this step's products without waiting for memory.  outs is a multiple of 8, grad aligned to
-// 16 bytes, and there are 16 values at least.
+// 16 bytes, and a row has 16 values at least.
 //
-// 8192 x 11008 x 4096 bf16: 732 us, 1.0 PFLOP/s (a library's bf16 product of these operands in this layout, the values widened
-// beforehand: 0.89); a step takes 3900 cycles, of which the matrix units are busy for 2048, LDS for 1200 and the conversion's
-// vector instructions for 1200; 688 tiles fill 2.7 of 3 rounds.  A raised wave priority around the products changes nothing.
+// 8192 x 11008 x 4096 bf16: 683 us, 1.08 PFLOP/s (a library's bf16 product of these operands in this layout, the values widened
+// beforehand: 0.89); a step takes 3700 cycles, of which the matrix units are busy for 2048, LDS for 1200 and vector instructions for
+// 1000, most of them the conversion (707 us with a scalar part twice as long, 732 us with eleven instructions for four values
+// instead of ten); 688 tiles fill 2.7 of 3 rounds.  A raised wave priority around the products changes nothing.
 template <int DT>
 __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p) {
   using T = typename Elem<DT>::type;
@@ -987,12 +985,15 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
     for (int j = 0; j < kC; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
 
   // Gradients: a wave's copy fills two rows of LDS; the sources follow the swizzle.  Columns behind the matrix come from the
-  // next row (or not at all, behind the last) and end in sums that are not stored.
-  const int width = (int)(p.stride - n0 < kTile ? p.stride - n0 : kTile);
+  // next row (or not at all, behind the last) and end in sums that are not stored.  What the last step has less than the
+  // others is worked out once and chosen inside the loop: computed there it was 4 % of the time.
+  const int last_rows = (int)(p.rows - (int64_t)(all - 1) * kRows);
+  auto rows_of = [&](int step) OPTIMI_INLINE { return step + 1 == all ? last_rows : kRows; };
+  const uint32_t width = (uint32_t)(p.stride - n0 < kTile ? p.stride - n0 : kTile);
   auto copy = [&](int step, short* g) OPTIMI_INLINE {
-    const int64_t m0 = (int64_t)step * kRows;
-    const int rows = (int)(p.rows - m0 < kRows ? p.rows - m0 : kRows);
-    const Buffer from = buffer_of((const T*)p.grad + m0 * p.stride + n0, ((int64_t)(rows - 1) * p.stride + width) * 2);
+    const T* base = (const T*)p.grad + (int64_t)step * kRows * p.stride + n0;
+    const uint32_t bytes = ((uint32_t)(rows_of(step) - 1) * (uint32_t)p.stride + width) * 2;  // below 2^31: see kMostWidth
+    const Buffer from = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(base), 0, (int)bytes, 0x00020000);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int place = i * 512 + threadIdx.x;
@@ -1002,24 +1003,27 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
     }
   };
   // Values: a lane has 16 neighbours of two rows.  Rows behind the last are the last one again, under a scale of 0;
-  // columns behind the matrix are never used.  A piece that would run over the end of all values is loaded from a little
-  // before, and shifted into its place when it is converted.
+  // columns behind the matrix are never used.  A piece that would run over the end of all values - in the last step only, the
+  // others have a row of 16 values at least behind them - is loaded from a little before, and shifted into its place
+  // when it is converted.
   const int64_t total = p.rows * p.cols;
   const int at_row = threadIdx.x / 16, at_col = threadIdx.x % 16;
   const uint32_t col = (uint32_t)c0 + (c0 + at_col * 16 < p.cols ? at_col * 16 : 0);
   u32x4 vq[2][kPieces];
   float sq[2][kPieces];
+  const int64_t last_first = (int64_t)(all - 1) * kRows * p.cols, last_start = last_first < total - 16 ? last_first : total - 16;
+  const uint32_t last_limit = (uint32_t)(total - 16 - last_start);
   auto place_of = [&](int step, int i, int64_t& start, uint32_t& limit) OPTIMI_INLINE {
-    const int64_t m0 = (int64_t)step * kRows, first = m0 * p.cols;
-    start = first < total - 16 ? first : total - 16;
-    const int64_t left = total - 16 - start;
-    limit = (uint32_t)(left < 0x7fffffff ? left : 0x7fffffff);
-    const int rows = (int)(p.rows - m0 < kRows ? p.rows - m0 : kRows), row = at_row + i * 32;
+    const int64_t first = (int64_t)step * kRows * p.cols;
+    const bool is_last = step + 1 == all;
+    start = is_last ? last_start : first;
+    limit = is_last ? last_limit : 0x7fffffffu;
+    const int rows = rows_of(step), row = at_row + i * 32;
     return (uint32_t)(row < rows ? row : rows - 1) * (uint32_t)p.cols + col + (uint32_t)(first - start);
   };
   auto load = [&](int step, u32x4 (&v)[kPieces], float (&s)[kPieces]) OPTIMI_INLINE {
     const int64_t m0 = (int64_t)step * kRows;
-    const int rows = (int)(p.rows - m0 < kRows ? p.rows - m0 : kRows);
+    const int rows = rows_of(step);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       int64_t start;
@@ -1031,7 +1035,7 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
     }
   };
   auto shift = [&](int step, u32x4 (&v)[kPieces], float (&s)[kPieces]) OPTIMI_INLINE {  // the very last step only
-    const int rows = (int)(p.rows - (int64_t)step * kRows);
+    const int rows = rows_of(step);
 #pragma unroll
     for (int i = 0; i < kPieces; ++i) {
       int64_t start;
