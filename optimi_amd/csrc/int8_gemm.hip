@@ -759,7 +759,7 @@ __device__ __forceinline__ void store_sums(const WeightGradArgs& p, const f32x4 
 // the step before theirs is multiplied, and written to LDS.  fp32 gradients are multiplied by their row's scale and split into
 // three bf16 pieces, so that their products are exact and cost three times as many instructions; the values are
 // whole numbers there.  NARROW: rows are shorter than a piece of a load, every load looks at the borders.
-// fp32 1000 x 4096 x 1023 with bias: 35 us; a step of 64 rows takes 1.7 us, of which the matrix instructions need 0.7 and the
+// fp32 1000 x 4096 x 1023 with bias: 34.5 us; a step of 64 rows takes 1.7 us, of which the matrix instructions need 0.7 and the
 // cutting into pieces about as much.  bf16 2048 x 2048 x 2048: 28 us, 0.65 us a step.
 template <int DT, bool NARROW>
 __global__ void __launch_bounds__(512) weight_grad_kernel(WeightGradArgs p) {
@@ -958,10 +958,10 @@ __global__ void __launch_bounds__(512) weight_grad_kernel(WeightGradArgs p) {
 // step's values can be spread over this step's products without waiting for memory.  outs is a multiple of 8, grad aligned to
 // 16 bytes, and a row has 16 values at least.
 //
-// 8192 x 11008 x 4096 bf16: 683 us, 1.08 PFLOP/s (a library's bf16 product of these operands in this layout, the values widened
-// beforehand: 0.89); a step takes 3700 cycles, of which the matrix units are busy for 2048, LDS for 1200 and vector instructions for
-// 1000, most of them the conversion (707 us with a scalar part twice as long, 732 us with eleven instructions for four values
-// instead of ten); 688 tiles fill 2.7 of 3 rounds.  A raised wave priority around the products changes nothing.
+// 8192 x 11008 x 4096 bf16: 676 us, 1.09 PFLOP/s (a library's bf16 product of these operands in this layout, the values widened
+// beforehand: 0.89); a step takes 3900 busy cycles by the counters, of which the matrix units are busy for 2048, LDS for 1300 (a
+// fifth of them bank conflicts) and vector instructions for 1000, two thirds of them the conversion: ten for four values (with eleven, and
+// the last step's borders worked out in every step, 735 us); 688 tiles fill 2.7 of 3 rounds.  A raised wave priority around the products changes nothing.
 template <int DT>
 __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p) {
   using T = typename Elem<DT>::type;
@@ -986,7 +986,7 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
 
   // Gradients: a wave's copy fills two rows of LDS; the sources follow the swizzle.  Columns behind the matrix come from the
   // next row (or not at all, behind the last) and end in sums that are not stored.  What the last step has less than the
-  // others is worked out once and chosen inside the loop: computed there it was 4 % of the time.
+  // others is worked out once and chosen inside the loop: 683 us instead of 707 at 8192 x 11008 x 4096.
   const int last_rows = (int)(p.rows - (int64_t)(all - 1) * kRows);
   auto rows_of = [&](int step) OPTIMI_INLINE { return step + 1 == all ? last_rows : kRows; };
   const uint32_t width = (uint32_t)(p.stride - n0 < kTile ? p.stride - n0 : kTile);
