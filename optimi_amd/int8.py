@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import math
 import warnings
+from contextlib import nullcontext
 from typing import Iterable, Sequence
 
 import torch
@@ -87,10 +88,12 @@ def _product(values, scales, weight, bias, dtype):
 
 
 def _times_weight(grad: Tensor, weight: Tensor, plus: Tensor | None = None) -> Tensor:
-    """``grad @ weight (+ plus)`` as one product of two matrices, whatever grad's dimensions and strides."""
+    """``grad @ weight (+ plus)`` as one product of two matrices, whatever grad's dimensions and strides, in their own
+    type: a backward pass may be called inside ``torch.autocast``, which would turn them into another one."""
     shape, (n, k) = grad.shape[:-1], weight.shape
     grad = grad.reshape(math.prod(shape), n)
-    out = grad.mm(weight) if plus is None else torch.addmm(plus.view(grad.shape[0], k), grad, weight)
+    with torch.autocast("cuda", enabled=False) if torch.is_autocast_enabled("cuda") else nullcontext():
+        out = grad.mm(weight) if plus is None else torch.addmm(plus.view(grad.shape[0], k), grad, weight)
     return out.view(*shape, k)
 
 

@@ -1,0 +1,54 @@
+"""The int8 operators and layers at the edges of what they allow, each against the operators' 64-bit forms or against the same
+operators called one by one."""
+
+import pytest
+import torch
+
+import int8_ref as R
+import optimi_amd as optimi
+from test_hip_int8 import norm_layers, rand
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------------- autocast around the backward pass
+
+@pytest.mark.parametrize("cast", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("dtype", R.DTYPES, ids=R.IDS)
+def test_backward_inside_autocast_is_that_outside(hip_device, dtype, cast):
+    """Layers that ran outside of autocast (or in a region where it is off) give the same gradients wherever backward() is called."""
+    m, k, outs = 11, 48, (24, 40)
+    x, r, nw, ws, bs = norm_layers(dtype, m, k, outs)
+    gs = [rand((m, n), dtype, 60 + n, 1e-2).to(hip_device) for n in outs]
+    results = []
+    for inside in (False, True):
+        leaf = lambda t: t.to(hip_device).requires_grad_()  # noqa: E731
+        lx, lr, ln, lw, lb = leaf(x), leaf(r), leaf(nw), [leaf(w) for w in ws], leaf(bs[1])
+        y = optimi.int8_linear(lx, lw[0])
+        ys, h = optimi.add_rms_norm_int8_linear(lx, ln, lw, biases=[None, lb], residual=lr)
+        with torch.autocast("cuda", dtype=cast, enabled=inside):
+            torch.autograd.backward([y, *ys, h], [gs[0], *gs, h.detach()])
+        results.append([t.grad for t in (lx, lr, ln, *lw, lb)])
+    for a, b in zip(*results):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("cast", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_a_whole_step_inside_autocast(hip_device, cast):
+    m, k, outs = 11, 48, (24, 40)
+    x, r, nw, ws, _ = norm_layers(torch.float32, m, k, outs)
+    results = []
+    for inside in (False, True):
+        leaf = lambda t: t.to(hip_device).requires_grad_()  # noqa: E731
+        lx, lr, ln, lw = leaf(x), leaf(r), leaf(nw), [leaf(w) for w in ws]
+        with torch.autocast("cuda", dtype=cast):
+            y = optimi.int8_linear(lx, lw[0])
+            (a, b), h = optimi.add_rms_norm_int8_linear(lx, ln, lw, residual=lr)
+            loss = y.float().square().mean() + a.float().square().mean() + b.float().square().mean() + h.float().square().mean()
+            if inside:
+                loss.backward()
+        if not inside:
+            loss.backward()
+        results.append([t.grad for t in (lx, lr, ln, *lw)])
+    for a, b in zip(*results):
+        assert a.dtype == torch.float32 and torch.equal(a, b)
