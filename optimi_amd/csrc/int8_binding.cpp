@@ -54,11 +54,15 @@ at::DimVector with_cols(const Tensor& t, int64_t cols) {
 }
 
 // The calls are short, and on small inputs the host's part of them is what counts: tensors are made by the allocator's own
-// function instead of through the dispatcher, and a contiguous one is taken as it is.
+// function instead of through the dispatcher, and a contiguous one is taken as it is, unless it carries the lazy negative bit: then
+// what lies in memory has the opposite sign.
 Tensor make(at::IntArrayRef sizes, at::ScalarType type, const Tensor& like) {
   return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
 }
-Tensor dense(const Tensor& t) { return t.is_contiguous() ? t : t.contiguous(); }
+Tensor dense(const Tensor& t) {
+  if (t.is_neg()) return t.resolve_neg().contiguous();
+  return t.is_contiguous() ? t : t.contiguous();
+}
 
 // values [..., cols] with one scale per row
 Tensor check_pair(const Tensor& values, const Tensor& scales, const char* name) {

@@ -11,6 +11,36 @@ from test_hip_int8 import norm_layers, rand
 pytestmark = pytest.mark.gpu
 
 
+# ---------------------------------------------------------------------------------- the lazy negative bit
+
+def turned(t):
+    """The same numbers, stored with the opposite sign under the negative bit; contiguous."""
+    view = torch._neg_view(-t)
+    assert view.is_neg() and view.is_contiguous() and torch.equal(view, t)
+    return view
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES, ids=R.IDS)
+def test_tensors_with_the_negative_bit(hip_device, dtype):
+    m, n, k = 9, 24, 40
+    x, r, g, w, b, nw = (rand(s, dtype, i).to(hip_device) for i, s in enumerate([(m, k), (m, k), (m, n), (n, k), (n,), (k,)]))
+    q, s = optimi.int8_quantize(x)
+    wq, ws = optimi.int8_quantize(w)
+    _, _, h, rstd = optimi.add_rms_norm_int8(x, nw, residual=r)
+    calls = {
+        "quantize": (lambda f: optimi.int8_quantize(f(x))),
+        "dequantize": (lambda f: (optimi.int8_dequantize(f(q), f(s), dtype),)),
+        "matmul": (lambda f: (optimi.int8_matmul(f(q), f(s), f(wq), f(ws), bias=f(b), dtype=dtype),)),
+        "weight gradient": (lambda f: optimi.int8_weight_grad(f(g), f(q), f(s), bias=True)),
+        "norm": (lambda f: optimi.add_rms_norm_int8(f(x), f(nw), residual=f(r))),
+        "norm alone": (lambda f: optimi.add_rms_norm_int8(f(x), f(nw))),
+        "norm backward": (lambda f: optimi.add_rms_norm_int8_backward(f(x), f(h), f(rstd), f(nw), grad_h=f(r))),
+    }
+    for name, call in calls.items():
+        for got, want in zip(call(turned), call(lambda t: t)):
+            assert torch.equal(got, want), name
+
+
 # ---------------------------------------------------------------------------------- autocast around the backward pass
 
 @pytest.mark.parametrize("cast", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
