@@ -201,14 +201,21 @@ def _is_norm_of(norm: nn.Module, layer: nn.Module) -> bool:
             and tuple(norm.normalized_shape) == (layer.in_features,) and not _has_hooks(norm) and not _has_hooks(layer))
 
 
+def _types_fit(x: Tensor, norm: nn.Module, layer: nn.Module) -> bool:
+    """Whether the operators take these types together; torch's own modules take more of them."""
+    autocast = torch.is_autocast_enabled("cuda")
+    dtype = torch.get_autocast_dtype("cuda") if autocast else x.dtype
+    return norm.weight.dtype in (dtype, torch.float32) and (autocast or layer.weight.dtype == dtype)
+
+
 class _Int8Sequential(nn.Sequential):
-    """Runs an RMSNorm that is directly followed by an Int8Linear as one node."""
+    """Runs an RMSNorm that is directly followed by an Int8Linear as one node, where their types allow it."""
 
     def forward(self, x):
         modules = list(self)
         i = 0
         while i < len(modules):
-            if i + 1 < len(modules) and _is_norm_of(modules[i], modules[i + 1]):
+            if i + 1 < len(modules) and _is_norm_of(modules[i], modules[i + 1]) and _types_fit(x, modules[i], modules[i + 1]):
                 norm, layer = modules[i], modules[i + 1]
                 # nn.RMSNorm without an eps adds that of the type it computes in
                 eps = torch.finfo(torch.float32).eps if norm.eps is None else norm.eps

@@ -3,6 +3,7 @@ operators called one by one."""
 
 import pytest
 import torch
+from torch import nn
 
 import int8_ref as R
 import optimi_amd as optimi
@@ -82,3 +83,15 @@ def test_a_whole_step_inside_autocast(hip_device, cast):
         results.append([t.grad for t in (lx, lr, ln, *lw)])
     for a, b in zip(*results):
         assert a.dtype == torch.float32 and torch.equal(a, b)
+
+
+# ---------------------------------------------------------------------------------- sequences
+
+def test_a_sequence_of_mixed_types_runs_as_it_did(hip_device):
+    """A bf16 norm in front of an fp32 layer on fp32 input: torch takes it, so the prepared sequence has to."""
+    plain = nn.Sequential(nn.RMSNorm(48, eps=1e-5).to(torch.bfloat16), nn.Linear(48, 24)).to(hip_device)
+    x = rand((7, 48), torch.float32, 1).to(hip_device)
+    normed = plain[0](x)
+    assert plain(x).dtype == torch.float32
+    optimi.prepare_for_int8_linear(plain)
+    assert torch.equal(plain(x), optimi.int8_linear(normed, plain[1].weight, plain[1].bias))

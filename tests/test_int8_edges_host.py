@@ -1,0 +1,59 @@
+"""What the int8 operators refuse and what a prepared model runs as before, at the edges; no GPU is touched."""
+
+import pytest
+import torch
+from torch import nn
+
+import optimi_amd as optimi
+from optimi_amd import int8
+
+
+# ---------------------------------------------------------------------------------- which modules run as one node
+
+@pytest.fixture
+def ran(monkeypatch):
+    """Torch operations in the operators' place; records whether a prepared sequence ran a layer by itself or with its norm."""
+    calls = []
+
+    def linear(x, weight, bias=None):
+        calls.append("linear")
+        return nn.functional.linear(x, weight, bias)
+
+    def norm(x, weight, residual=None, eps=1e-6):
+        calls.append("fused")
+        return nn.functional.rms_norm(x, weight.shape, weight, eps), torch.ones(len(x)), x, torch.ones(len(x))
+
+    monkeypatch.setattr(int8, "int8_linear", linear)
+    monkeypatch.setattr(int8, "add_rms_norm_int8", norm)
+    monkeypatch.setattr(int8, "int8_quantize", lambda x: (x, None))
+    monkeypatch.setattr(int8, "int8_matmul", lambda x, sx, w, sw, bias, dtype: nn.functional.linear(x, w, bias))
+    monkeypatch.setattr(int8.backend, "check_supported", lambda t: None)
+    return calls
+
+
+def sequence(norm_dtype=torch.float32, layer_dtype=torch.float32):
+    torch.manual_seed(0)
+    plain = nn.Sequential(nn.RMSNorm(8, eps=1e-5).to(norm_dtype), nn.Linear(8, 4).to(layer_dtype))
+    return optimi.prepare_for_int8_linear(plain)
+
+
+@pytest.mark.parametrize("x,norm,layer,want", [
+    (torch.float32, torch.float32, torch.float32, "fused"),
+    (torch.bfloat16, torch.bfloat16, torch.bfloat16, "fused"),
+    (torch.float32, torch.bfloat16, torch.float32, "linear"),
+    (torch.float32, torch.float16, torch.float32, "linear"),
+])
+def test_the_types_decide_whether_a_norm_and_its_layer_are_one(ran, x, norm, layer, want):
+    model = sequence(norm, layer)
+    plain = nn.Sequential(*(optimi.remove_int8_linear(sequence(norm, layer))))
+    t = torch.randn(3, 8).to(x)
+    y, y0 = model(t), plain(t)
+    assert ran == [want]
+    assert y.dtype == y0.dtype and torch.allclose(y.float(), y0.float(), rtol=0.02, atol=0.02)
+
+
+def test_types_that_torch_refuses_are_refused(ran):
+    model = sequence(torch.float32, torch.bfloat16)
+    with pytest.raises(RuntimeError):
+        model(torch.randn(3, 8))
+    assert "fused" not in ran
