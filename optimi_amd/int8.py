@@ -134,6 +134,8 @@ def int8_linear(x: Tensor, weight: Tensor, bias: Tensor | None = None) -> Tensor
 
 
 class _AddRmsNormInt8Linear(torch.autograd.Function):
+    """The norm in x's type and the layers in theirs, which need not be the same."""
+
     @staticmethod
     def forward(ctx, x, residual, norm_weight, eps, *layers):
         weights, biases = layers[: len(layers) // 2], layers[len(layers) // 2:]
@@ -141,7 +143,7 @@ class _AddRmsNormInt8Linear(torch.autograd.Function):
         ctx.set_materialize_grads(False)
         ctx.with_residual = residual is not None
         ctx.save_for_backward(values, scales, h, rstd, norm_weight, *weights)
-        outs = tuple(_product(values, scales, w, b, x.dtype) for w, b in zip(weights, biases))
+        outs = tuple(_product(values, scales, w, b, w.dtype) for w, b in zip(weights, biases))
         return (h, *outs) if ctx.with_residual else outs
 
     @staticmethod
@@ -163,7 +165,7 @@ class _AddRmsNormInt8Linear(torch.autograd.Function):
                 dws[i] = dw if need_w else None
         dx, dnorm = grad_h, None
         if dy is not None:
-            dx, dnorm = add_rms_norm_int8_backward(dy, h, rstd, norm_weight, grad_h)
+            dx, dnorm = add_rms_norm_int8_backward(dy.to(h.dtype), h, rstd, norm_weight, grad_h)
         return (dx if need_x else None, dx if need_residual else None, dnorm if need_norm else None, None, *dws, *dbs)
 
 
@@ -203,9 +205,18 @@ def _is_norm_of(norm: nn.Module, layer: nn.Module) -> bool:
 
 def _types_fit(x: Tensor, norm: nn.Module, layer: nn.Module) -> bool:
     """Whether the operators take these types together; torch's own modules take more of them."""
-    autocast = torch.is_autocast_enabled("cuda")
-    dtype = torch.get_autocast_dtype("cuda") if autocast else x.dtype
-    return norm.weight.dtype in (dtype, torch.float32) and (autocast or layer.weight.dtype == dtype)
+    return (x.dtype in backend.SUPPORTED_DTYPES and norm.weight.dtype in (x.dtype, torch.float32)
+            and (layer.weight.dtype == x.dtype or torch.is_autocast_enabled("cuda")))
+
+
+def _norm_layer(x: Tensor, norm: nn.Module, layer: nn.Module) -> Tensor:
+    """Under ``torch.autocast`` the layer is cast and the norm is not: its input may be a residual stream of more bits."""
+    weight, bias = _autocast(layer.weight, layer.bias)
+    _check_linear(weight, weight, bias)
+    # nn.RMSNorm without an eps adds that of the type it computes in
+    eps = torch.finfo(torch.float32).eps if norm.eps is None else norm.eps
+    (y,) = _AddRmsNormInt8Linear.apply(x, None, norm.weight, eps, weight, bias)
+    return y
 
 
 class _Int8Sequential(nn.Sequential):
@@ -216,10 +227,7 @@ class _Int8Sequential(nn.Sequential):
         i = 0
         while i < len(modules):
             if i + 1 < len(modules) and _is_norm_of(modules[i], modules[i + 1]) and _types_fit(x, modules[i], modules[i + 1]):
-                norm, layer = modules[i], modules[i + 1]
-                # nn.RMSNorm without an eps adds that of the type it computes in
-                eps = torch.finfo(torch.float32).eps if norm.eps is None else norm.eps
-                (x,), _ = add_rms_norm_int8_linear(x, norm.weight, [layer.weight], [layer.bias], eps=eps)
+                x = _norm_layer(x, modules[i], modules[i + 1])
                 i += 2
             else:
                 x = modules[i](x)
@@ -234,7 +242,8 @@ _MODULES_ATTR = "_int8_linear_modules"
 def prepare_for_int8_linear(model: nn.Module, skip: Iterable[str] = ()) -> nn.Module:
     """Makes every ``nn.Linear`` of ``model`` (in place; itself included) an ``Int8Linear``, except those whose qualified
     name contains one of the strings in ``skip``, and lets an ``nn.RMSNorm`` directly before one in an ``nn.Sequential``
-    hand it int8 values.  Subclasses of these modules are left alone.  Parameters stay the same objects: optimizers
+    hand it int8 values (under ``torch.autocast`` the norm takes its input as it comes, the layer runs in the autocast type).  Subclasses
+    of these modules are left alone.  Parameters stay the same objects: optimizers
     built before or after, gradient release and checkpoints work as they did.  ``ValueError`` if the model is prepared
     already or holds no such layer.  Undo with ``remove_int8_linear``."""
     if isinstance(skip, str):

@@ -95,3 +95,27 @@ def test_a_sequence_of_mixed_types_runs_as_it_did(hip_device):
     assert plain(x).dtype == torch.float32
     optimi.prepare_for_int8_linear(plain)
     assert torch.equal(plain(x), optimi.int8_linear(normed, plain[1].weight, plain[1].bias))
+
+
+# ---------------------------------------------------------------------------------- a sequence under autocast
+
+@pytest.mark.parametrize("cast", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+def test_the_norm_of_a_sequence_sees_all_bits_under_autocast(hip_device, cast):
+    """The residual stream stays in float32 up to the norm; only the layer runs in the autocast type."""
+    m, k, n = 13, 96, 40
+    model = nn.Sequential(nn.RMSNorm(k, eps=1e-5), nn.Linear(k, n)).to(hip_device)
+    optimi.prepare_for_int8_linear(model)
+    x = rand((m, k), torch.float32, 2).to(hip_device).requires_grad_()
+    with torch.autocast("cuda", dtype=cast):
+        y = model(x)
+    g = rand((m, n), cast, 3, 1e-2).to(hip_device)
+    y.backward(g)
+    with torch.no_grad():
+        w, b = model[1].weight.to(cast), model[1].bias.to(cast)
+        values, scales, h, rstd = optimi.add_rms_norm_int8(x, model[0].weight, eps=1e-5)
+        want = optimi.int8_matmul(values, scales, *optimi.int8_quantize(w), bias=b, dtype=cast)
+        assert y.dtype == cast and torch.equal(y, want)
+        dx, dn = optimi.add_rms_norm_int8_backward((g @ w).float(), h, rstd, model[0].weight)
+        assert torch.equal(x.grad, dx) and torch.equal(model[0].weight.grad, dn)
+        dw, db = optimi.int8_weight_grad(g, values, scales, bias=True)
+        assert torch.equal(model[1].weight.grad, dw.float()) and torch.equal(model[1].bias.grad, db.float())
