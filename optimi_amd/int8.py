@@ -24,6 +24,7 @@ from typing import Iterable, Sequence
 import torch
 from torch import Tensor, nn
 from torch.autograd.function import once_differentiable
+from torch.nn.modules import module as nn_module
 
 from . import backend
 
@@ -194,13 +195,17 @@ class Int8Linear(nn.Linear):
         return int8_linear(x, self.weight, self.bias)
 
 
-def _has_hooks(module: nn.Module) -> bool:
-    return bool(module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks)
+def _only_forward(module: nn.Module) -> bool:
+    """Whether a call of the module is its class's forward() and nothing else: no hooks of its own or on all modules, no
+    forward() of the instance, not compiled."""
+    return not (module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks
+                or nn_module._global_forward_hooks or nn_module._global_forward_pre_hooks or nn_module._global_backward_hooks
+                or nn_module._global_backward_pre_hooks or "forward" in module.__dict__ or module._compiled_call_impl is not None)
 
 
 def _is_norm_of(norm: nn.Module, layer: nn.Module) -> bool:
     return (type(norm) is nn.RMSNorm and type(layer) is Int8Linear and norm.elementwise_affine
-            and tuple(norm.normalized_shape) == (layer.in_features,) and not _has_hooks(norm) and not _has_hooks(layer))
+            and tuple(norm.normalized_shape) == (layer.in_features,) and _only_forward(norm) and _only_forward(layer))
 
 
 def _types_fit(x: Tensor, norm: nn.Module, layer: nn.Module) -> bool:

@@ -57,3 +57,45 @@ def test_types_that_torch_refuses_are_refused(ran):
     with pytest.raises(RuntimeError):
         model(torch.randn(3, 8))
     assert "fused" not in ran
+
+
+# ---------------------------------------------------------------------------------- modules that someone else has to see called
+
+@pytest.mark.parametrize("at", [0, 1])
+def test_a_forward_of_its_own_is_called(ran, at):
+    """Libraries that offload or move modules replace the instance's forward."""
+    model = sequence()
+    inner, seen = model[at].forward, []
+
+    def wrapped(x):
+        seen.append(at)
+        return inner(x)
+
+    model[at].forward = wrapped
+    x = torch.randn(3, 8)
+    model(x)
+    assert seen == [at] and ran == ["linear"]
+    del model[at].forward
+    model(x)
+    assert ran == ["linear", "fused"]
+
+
+def test_a_compiled_module_is_called(ran):
+    model, seen = sequence(), []
+    model[0]._compiled_call_impl = lambda x: seen.append(1) or x
+    model(torch.randn(3, 8))
+    assert seen == [1] and ran == ["linear"]
+
+
+@pytest.mark.parametrize("register", [nn.modules.module.register_module_forward_hook, nn.modules.module.register_module_forward_pre_hook,
+                                      nn.modules.module.register_module_full_backward_hook, nn.modules.module.register_module_full_backward_pre_hook])
+def test_hooks_on_all_modules_see_every_module(ran, register):
+    model, seen = sequence(), []
+    handle = register(lambda module, *args: seen.append(type(module).__name__))
+    try:
+        model(torch.randn(3, 8, requires_grad=True)).sum().backward()
+    finally:
+        handle.remove()
+    assert "RMSNorm" in seen and "Int8Linear" in seen and ran == ["linear"]
+    model(torch.randn(3, 8))
+    assert ran == ["linear", "fused"]
