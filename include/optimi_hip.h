@@ -378,7 +378,8 @@ int optimi_hip_int8_matmul(const int8_t* a, const float* a_scales, const int8_t*
  * is not NULL.  grad [rows, outs], values [rows, cols], weight_grad [outs, cols]; all but values and scales are of
  * `dtype`.  Products of bf16 and fp16 gradients are formed with values[r][k] * scales[r] rounded to that type (exact
  * for this library's scales), those of fp32 gradients without rounding, where grad * scale lies between
- * 2^-110 and the largest float; sums are fp32.  rows = 0 writes zeros. */
+ * 2^-110 and the largest float; sums are fp32.  rows = 0 writes zeros; cols = 0 leaves the
+ * bias gradient, for which values, scales and weight_grad may be NULL. */
 int64_t optimi_hip_int8_weight_grad_workspace(int64_t rows, int64_t outs, int64_t cols, int dtype, int with_bias);
 int optimi_hip_int8_weight_grad(const void* grad, const int8_t* values, const float* scales, int64_t rows, int64_t outs,
                                 int64_t cols, int dtype, void* weight_grad, void* bias_grad, void* workspace,

@@ -160,6 +160,20 @@ std::tuple<Tensor, std::optional<Tensor>> int8_weight_grad(const Tensor& grad_, 
   return {dw, db};
 }
 
+// the column sums of grad, which need no checkpoint
+Tensor int8_bias_grad(const Tensor& grad_) {
+  check_device(grad_, grad_, "the gradient");
+  const int dtype = dtype_code(grad_.scalar_type(), "the gradient");
+  const Rows g = rows_of(grad_, "the gradient");
+  c10::hip::HIPGuardMasqueradingAsCUDA guard(grad_.device());
+  const Tensor grad = dense(grad_);
+  Tensor db = make({g.cols}, grad.scalar_type(), grad);
+  const Tensor work = workspace(optimi_hip_int8_weight_grad_workspace(g.rows, g.cols, 0, dtype, 1), grad, "optimi_hip_int8_weight_grad");
+  check_status(optimi_hip_int8_weight_grad(grad.data_ptr(), nullptr, nullptr, g.rows, g.cols, 0, dtype, nullptr, db.data_ptr(), pointer(work), current_stream()),
+               "optimi_hip_int8_weight_grad");
+  return db;
+}
+
 int norm_weight_code(const Tensor& weight, const Tensor& x, int64_t cols) {
   check_device(x, weight, "the norm's weight");
   TORCH_CHECK(weight.scalar_type() == x.scalar_type() || weight.scalar_type() == at::kFloat, "optimi_amd: the norm's weight has dtype ",
@@ -229,6 +243,7 @@ void bind_int8(py::module& mod) {
   mod.def("int8_dequantize", &int8_dequantize);
   mod.def("int8_matmul", &int8_matmul);
   mod.def("int8_weight_grad", &int8_weight_grad);
+  mod.def("int8_bias_grad", &int8_bias_grad);
   mod.def("add_rms_norm_int8", &add_rms_norm_int8);
   mod.def("add_rms_norm_int8_backward", &add_rms_norm_int8_backward);
 }

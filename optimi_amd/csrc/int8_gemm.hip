@@ -1407,7 +1407,7 @@ int optimi_hip_int8_weight_grad(const void* grad, const int8_t* values, const fl
   if (int rc = check_shape(rows, cols)) return rc;
   if (outs > kMostWidth || cols > kMostWidth) return OPTIMI_ERR_SIZE;
   if (outs == 0) return 0;
-  if ((cols && !weight_grad) || (rows && (!grad || !scales || (cols && !values)))) return OPTIMI_ERR_NULL;
+  if ((cols && !weight_grad) || (rows && (!grad || (cols && (!scales || !values))))) return OPTIMI_ERR_NULL;
   const int64_t size = elem_bytes(dtype);
   if (!aligned_to(grad, size) || !aligned_to(scales, 4) || !aligned_to(weight_grad, size) || !aligned_to(bias_grad, size) || !aligned_to(workspace, 16))
     return OPTIMI_ERR_ALIGN;

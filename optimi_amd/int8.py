@@ -98,12 +98,18 @@ def _times_weight(grad: Tensor, weight: Tensor, plus: Tensor | None = None) -> T
     return out.view(*shape, k)
 
 
+def _parameter_grads(grad, values, scales, need_weight, need_bias):
+    if need_weight:
+        return backend.ext().int8_weight_grad(grad, values, scales, need_bias)
+    return None, backend.ext().int8_bias_grad(grad) if need_bias else None
+
+
 class _Int8Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
         values, scales = int8_quantize(x)
-        keep = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]  # without them the checkpoint is not needed
-        ctx.save_for_backward(weight, *((values, scales) if keep else (None, None)))
+        # the checkpoint is for the weight's gradient alone
+        ctx.save_for_backward(weight, *((values, scales) if ctx.needs_input_grad[1] else (None, None)))
         return _product(values, scales, weight, bias, x.dtype)
 
     @staticmethod
@@ -111,10 +117,7 @@ class _Int8Linear(torch.autograd.Function):
     def backward(ctx, grad):
         weight, values, scales = ctx.saved_tensors
         dx = _times_weight(grad, weight) if ctx.needs_input_grad[0] else None
-        dw = db = None
-        if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
-            dw, db = backend.ext().int8_weight_grad(grad, values, scales, ctx.needs_input_grad[2])
-        return dx, dw if ctx.needs_input_grad[1] else None, db
+        return dx, *_parameter_grads(grad, values, scales, *ctx.needs_input_grad[1:3])
 
 
 def _autocast(*tensors):
@@ -160,10 +163,7 @@ class _AddRmsNormInt8Linear(torch.autograd.Function):
                 continue
             if need_x or need_residual or need_norm:
                 dy = _times_weight(grad, weight, plus=dy)
-            need_w, need_b = ctx.needs_input_grad[4 + i], ctx.needs_input_grad[4 + n + i]
-            if need_w or need_b:
-                dw, dbs[i] = backend.ext().int8_weight_grad(grad, values, scales, need_b)
-                dws[i] = dw if need_w else None
+            dws[i], dbs[i] = _parameter_grads(grad, values, scales, ctx.needs_input_grad[4 + i], ctx.needs_input_grad[4 + n + i])
         dx, dnorm = grad_h, None
         if dy is not None:
             dx, dnorm = add_rms_norm_int8_backward(dy.to(h.dtype), h, rstd, norm_weight, grad_h)

@@ -7,7 +7,8 @@ from torch import nn
 
 import int8_ref as R
 import optimi_amd as optimi
-from test_hip_int8 import norm_layers, rand
+from optimi_amd import backend
+from test_hip_int8 import checkpoint, norm_layers, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -119,3 +120,44 @@ def test_the_norm_of_a_sequence_sees_all_bits_under_autocast(hip_device, cast):
         assert torch.equal(x.grad, dx) and torch.equal(model[0].weight.grad, dn)
         dw, db = optimi.int8_weight_grad(g, values, scales, bias=True)
         assert torch.equal(model[1].weight.grad, dw.float()) and torch.equal(model[1].bias.grad, db.float())
+
+
+# ---------------------------------------------------------------------------------- layers that are frozen in part
+
+@pytest.fixture
+def no_weight_grad(monkeypatch):
+    def refuse(*args):
+        raise AssertionError("a weight gradient that nobody asked for")
+
+    monkeypatch.setattr(backend.ext(), "int8_weight_grad", refuse)
+
+
+def kept_int8(y):
+    return [t for t in y.grad_fn.saved_tensors if t is not None and t.dtype == torch.int8]
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES, ids=R.IDS)
+@pytest.mark.parametrize("shape", [(0, 40), (1, 5), (5, 1000), (127, 300), (128, 2048), (129, 2049), (1000, 40), (300, 9001)], ids=lambda s: "x".join(map(str, s)))
+def test_a_bias_alone(hip_device, shape, dtype, no_weight_grad):
+    m, n = shape
+    x, w, g = rand((m, 24), dtype, 1).to(hip_device), rand((n, 24), dtype, 2).to(hip_device), rand((m, n), dtype, 3, 1e-2)
+    b = torch.zeros(n, dtype=dtype, device=hip_device, requires_grad=True)
+    y = optimi.int8_linear(x, w, b)
+    assert kept_int8(y) == [], "a bias gradient needs no checkpoint"
+    y.backward(g.to(hip_device))
+    R.close(b.grad, *R.column_sum(g, dtype), "bias")
+    grad, b.grad = b.grad, None
+    optimi.int8_linear(x, w, b).backward(g.to(hip_device).t().contiguous().t())
+    assert torch.equal(b.grad, grad)
+    b.grad = None
+    (y,), _ = optimi.add_rms_norm_int8_linear(x, torch.ones(24, dtype=dtype, device=hip_device), [w], biases=[b])
+    y.backward(g.to(hip_device))
+    assert torch.equal(b.grad, grad)
+
+
+def test_a_bias_alone_of_one_vector_and_of_a_sum(hip_device, no_weight_grad):
+    w, b = rand((40, 24), torch.float32, 1).to(hip_device), torch.zeros(40, device=hip_device, requires_grad=True)
+    optimi.int8_linear(rand((24,), torch.float32, 2).to(hip_device), w, b).sum().backward()
+    assert torch.equal(b.grad, torch.ones_like(b))
+    optimi.int8_linear(rand((3, 5, 24), torch.float32, 2).to(hip_device), w, b).sum().backward()
+    assert torch.equal(b.grad, torch.full_like(b, 16.0))
