@@ -146,7 +146,10 @@ class _AddRmsNormInt8Linear(torch.autograd.Function):
         values, scales, h, rstd = add_rms_norm_int8(x, norm_weight, residual, eps)
         ctx.set_materialize_grads(False)
         ctx.with_residual = residual is not None
-        ctx.save_for_backward(values, scales, h, rstd, norm_weight, *weights)
+        # the checkpoint is for the weights' gradients alone, the sum for the norm's
+        checkpoint = (values, scales) if any(ctx.needs_input_grad[4:4 + len(weights)]) else (None, None)
+        kept = (h, rstd, norm_weight) if any(ctx.needs_input_grad[:3]) else (None, None, None)
+        ctx.save_for_backward(*checkpoint, *kept, *weights)
         outs = tuple(_product(values, scales, w, b, w.dtype) for w, b in zip(weights, biases))
         return (h, *outs) if ctx.with_residual else outs
 

@@ -161,3 +161,43 @@ def test_a_bias_alone_of_one_vector_and_of_a_sum(hip_device, no_weight_grad):
     assert torch.equal(b.grad, torch.ones_like(b))
     optimi.int8_linear(rand((3, 5, 24), torch.float32, 2).to(hip_device), w, b).sum().backward()
     assert torch.equal(b.grad, torch.full_like(b, 16.0))
+
+
+# ---------------------------------------------------------------------------------- frozen layers behind a norm
+
+def test_frozen_layers_behind_a_trained_norm(hip_device, no_weight_grad):
+    x, r, nw, ws, _ = norm_layers(torch.bfloat16, 20, 64, (32, 48))
+    lx, ln = x.to(hip_device).requires_grad_(), nw.to(hip_device).requires_grad_()
+    ws = [w.to(hip_device) for w in ws]
+    (y0, y1), h = optimi.add_rms_norm_int8_linear(lx, ln, ws, residual=r.to(hip_device))
+    assert kept_int8(y0) == [], "without a weight gradient the checkpoint is not needed"
+    g0, g1 = torch.randn_like(y0), torch.randn_like(y1)
+    torch.autograd.backward([y0, y1], [g0, g1])
+    with torch.no_grad():
+        _, _, h, rstd = optimi.add_rms_norm_int8(lx, ln, residual=r.to(hip_device))
+        dx, dn = optimi.add_rms_norm_int8_backward(torch.addmm(g0 @ ws[0], g1, ws[1]), h, rstd, ln)
+    assert torch.equal(lx.grad, dx) and torch.equal(ln.grad, dn)
+
+
+def test_a_bias_alone_behind_a_norm(hip_device, no_weight_grad):
+    x, _, nw, ws, bs = norm_layers(torch.bfloat16, 20, 64, (32, 48))
+    lb = bs[1].to(hip_device).requires_grad_()
+    (y,), _ = optimi.add_rms_norm_int8_linear(x.to(hip_device), nw.to(hip_device), [ws[1].to(hip_device)], biases=[lb])
+    assert kept_int8(y) == []
+    g = torch.randn_like(y)
+    y.backward(g)
+    R.close(lb.grad, *R.column_sum(g.cpu(), torch.bfloat16), "bias")
+
+
+def test_one_of_two_layers_is_trained(hip_device):
+    x, _, nw, ws, bs = norm_layers(torch.bfloat16, 20, 64, (32, 48))
+    ln, lw, lb = nw.to(hip_device), [w.to(hip_device) for w in ws], bs[1].to(hip_device).requires_grad_()
+    lw[0].requires_grad_()
+    ys, _ = optimi.add_rms_norm_int8_linear(x.to(hip_device), ln, lw, biases=[None, lb])
+    assert len(kept_int8(ys[0])) == 1
+    assert [t.dtype for t in ys[0].grad_fn.saved_tensors if t is not None and t.shape == x.shape] == [torch.int8], "no gradient flows into the norm"
+    gs = [torch.randn_like(y) for y in ys]
+    torch.autograd.backward(ys, gs)
+    values, scales, _, _ = optimi.add_rms_norm_int8(x.to(hip_device), ln)
+    assert torch.equal(lw[0].grad, optimi.int8_weight_grad(gs[0], values, scales))
+    R.close(lb.grad, *R.column_sum(gs[1].cpu(), torch.bfloat16), "bias")
