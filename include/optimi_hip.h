@@ -350,7 +350,8 @@ int64_t optimi_hip_launch_limit(int64_t workgroups);
  * that holds an infinity or a NaN gets the scale NaN and zeros.  The products take any scales.
  *
  * All matrices are contiguous, rows < 2^31, cols <= 2^28 (outs and cols <= 2^24 for the weight
- * gradient), and a product has at most 2^22 tiles of 64 x 64 outputs or larger (OPTIMI_ERR_SIZE beyond).  Buffers need
+ * gradient), and a product has fewer than 2^24 tiles of 64 x 64 outputs (OPTIMI_ERR_SIZE beyond); where operands are
+ * aligned to 16 bytes larger tiles carry it further (OPTIMI_ERR_ALIGN where only aligned ones would fit).  Buffers need
  * only be aligned to their element size; outputs overlap neither inputs nor each other.  Workspaces are the caller's: as many bytes of device memory
  * as the _workspace function of the same name and sizes says (it returns a negative status for
  * sizes that the call would refuse), aligned to 16 bytes, not shared by calls that may

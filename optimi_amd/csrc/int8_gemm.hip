@@ -1185,7 +1185,8 @@ int by_dtype(int dtype, F f) {
 
 constexpr int64_t kMostWidth = 1 << 24;  // of a weight gradient: offsets inside a tile stay in 31 bits
 constexpr int64_t kMostSum = 131071;  // (-128)^2 times this stays below 2^31
-constexpr int64_t kMostTiles = 1 << 22;  // workgroups of a launch, at most 512 lanes each
+// A launch holds fewer than 2^32 lanes.
+inline bool launch_holds(int64_t workgroups, int lanes) { return workgroups < ((int64_t)1 << 32) / lanes; }
 
 // How a product is cut: the tile's size and the number of parts that the sum is split into.
 struct Cut {
@@ -1261,6 +1262,7 @@ inline int64_t padded(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 // Odd widths: large tiles are copied asynchronously and take padded copies of both operands.  Small ones can be loaded through registers,
 // at 0.45 us a step instead of 0.2; the copies cost a launch and 0.5 us per million bytes (measured: 42 x 216 x 3675 16.6 us through
 // registers, 13.3 us padded; 20 x 8000 x 8001 32 us, 38 us).
+inline int64_t vec_blocks(int64_t n, bool share) { return share ? (n + 3) / 4 : (n + 15) / 16; }
 struct MatmulPlan {
   bool vec;         // read off the weight
   bool pad;         // padded copies of both operands come first
@@ -1269,13 +1271,24 @@ struct MatmulPlan {
 };
 MatmulPlan matmul_plan(int64_t m, int64_t n, int64_t k) {
   MatmulPlan plan{};
-  plan.vec = m <= kMostVec;
+  plan.vec = m <= kMostVec && launch_holds(vec_blocks(n, false), 256);
   if (plan.vec) return plan;
   plan.cut = matmul_cut(m, n, k);
   plan.pad = k % 16 != 0 && (plan.cut.tile > 64 || 0.25 * (double)((k + kStep - 1) / kStep) > 2.0 + 0.5e-6 * (double)((m + n) * k));
   plan.pad_bytes = plan.pad ? (m + n) * padded(k) : 0;
   plan.partial_bytes = plan.cut.splits > 1 ? plan.cut.splits * m * n * 4 : 0;
   return plan;
+}
+
+inline int matmul_lanes(int tile) { return tile == 256 ? 512 : 256; }
+
+// The sizes that the call and its workspace function refuse.
+int matmul_sizes(int64_t m, int64_t n, int64_t k) {
+  if (int rc = check_shape(m, n)) return rc;
+  if (k < 0 || k > kMostSum) return OPTIMI_ERR_SIZE;
+  if (m == 0 || n == 0) return 0;
+  const MatmulPlan plan = matmul_plan(m, n, k);
+  return plan.vec || launch_holds(plan.cut.tiles * plan.cut.splits, matmul_lanes(plan.cut.tile)) ? 0 : (int)OPTIMI_ERR_SIZE;
 }
 
 struct WeightGradPlan {
@@ -1298,11 +1311,20 @@ WeightGradPlan weight_grad_plan(int64_t rows, int64_t outs, int64_t cols, int dt
   return plan;
 }
 
+constexpr int kWeightGradLanes = 512;
+int weight_grad_sizes(int64_t rows, int64_t outs, int64_t cols, int dtype, bool with_bias) {
+  if (int rc = check_shape(rows, outs)) return rc;
+  if (int rc = check_shape(rows, cols)) return rc;
+  if (outs > kMostWidth || cols > kMostWidth) return OPTIMI_ERR_SIZE;
+  if (outs == 0 || cols == 0) return 0;
+  const WeightGradPlan plan = weight_grad_plan(rows, outs, cols, dtype, with_bias);
+  return launch_holds(plan.cut.tiles * plan.cut.splits, kWeightGradLanes) ? 0 : (int)OPTIMI_ERR_SIZE;
+}
+
 template <int DT>
 int launch_vec(const MatmulArgs& args, hipStream_t stream) {
   const bool share = (args.n + 15) / 16 < 2 * kCus && args.k > 1024;
-  const int64_t blocks = share ? (args.n + 3) / 4 : (args.n + 15) / 16;
-  const dim3 grid((unsigned)blocks), block(256);
+  const dim3 grid((unsigned)vec_blocks(args.n, share)), block(256);
   auto go = [&](auto m) {
     constexpr int M = decltype(m)::value;
     if (share) matvec_kernel<DT, M, 4><<<grid, block, 0, stream>>>(args);
@@ -1328,8 +1350,7 @@ int pad_rows(const void* a, int64_t rows_a, const void* b, int64_t rows_b, int64
 extern "C" {
 
 int64_t optimi_hip_int8_matmul_workspace(int64_t m, int64_t n, int64_t k) {
-  if (int rc = check_shape(m, n)) return rc;
-  if (k < 0 || k > kMostSum) return OPTIMI_ERR_SIZE;
+  if (int rc = matmul_sizes(m, n, k)) return rc;
   if (m == 0 || n == 0) return 0;
   const MatmulPlan plan = matmul_plan(m, n, k);
   return plan.pad_bytes + plan.partial_bytes;
@@ -1338,8 +1359,7 @@ int64_t optimi_hip_int8_matmul_workspace(int64_t m, int64_t n, int64_t k) {
 int optimi_hip_int8_matmul(const int8_t* a, const float* a_scales, const int8_t* b, const float* b_scales, const void* bias, int64_t m, int64_t n,
                            int64_t k, int dtype, void* out, void* workspace, optimi_stream_t stream_) {
   if (!valid_dtype(dtype)) return OPTIMI_ERR_DTYPE;
-  if (int rc = check_shape(m, n)) return rc;
-  if (k < 0 || k > kMostSum) return OPTIMI_ERR_SIZE;
+  if (int rc = matmul_sizes(m, n, k)) return rc;
   if (m == 0 || n == 0) return 0;
   if (!a_scales || !b_scales || !out || (k && (!a || !b))) return OPTIMI_ERR_NULL;
   const int64_t size = elem_bytes(dtype);
@@ -1348,7 +1368,6 @@ int optimi_hip_int8_matmul(const int8_t* a, const float* a_scales, const int8_t*
   if (plan.pad_bytes + plan.partial_bytes > 0 && !workspace) return OPTIMI_ERR_NULL;
   hipStream_t stream = (hipStream_t)stream_;
   MatmulArgs args{a, a_scales, b, b_scales, bias, m, n, k, out, nullptr, 1, 0};
-  if (plan.vec && (n + 15) / 16 > 2 * kMostTiles) return OPTIMI_ERR_SIZE;
   if (plan.vec) return by_dtype(dtype, [&](auto dt) { return launch_vec<decltype(dt)::value>(args, stream); });
 
   Cut c = plan.cut;
@@ -1364,8 +1383,8 @@ int optimi_hip_int8_matmul(const int8_t* a, const float* a_scales, const int8_t*
   if (!aligned && c.tile > 64) {  // operands that start off the grid: tiles that go through registers are small ones
     c.tile = 64;
     c.tiles = tiles_of(m, n, 64);
+    if (!launch_holds(c.tiles * c.splits, matmul_lanes(64))) return OPTIMI_ERR_ALIGN;
   }
-  if (c.tiles * c.splits > kMostTiles) return OPTIMI_ERR_SIZE;
   args.partial = (int32_t*)((int8_t*)workspace + plan.pad_bytes);
   args.splits = c.splits;
   args.steps_per_split = c.steps_per_split;
@@ -1392,9 +1411,7 @@ int optimi_hip_int8_matmul(const int8_t* a, const float* a_scales, const int8_t*
 
 int64_t optimi_hip_int8_weight_grad_workspace(int64_t rows, int64_t outs, int64_t cols, int dtype, int with_bias) {
   if (!valid_dtype(dtype)) return OPTIMI_ERR_DTYPE;
-  if (int rc = check_shape(rows, outs)) return rc;
-  if (int rc = check_shape(rows, cols)) return rc;
-  if (outs > kMostWidth || cols > kMostWidth) return OPTIMI_ERR_SIZE;
+  if (int rc = weight_grad_sizes(rows, outs, cols, dtype, with_bias != 0)) return rc;
   if (outs == 0) return 0;
   const WeightGradPlan plan = weight_grad_plan(rows, outs, cols, dtype, with_bias != 0);
   return plan.pad_bytes + plan.partial_bytes + plan.bias_bytes;
@@ -1403,9 +1420,7 @@ int64_t optimi_hip_int8_weight_grad_workspace(int64_t rows, int64_t outs, int64_
 int optimi_hip_int8_weight_grad(const void* grad, const int8_t* values, const float* scales, int64_t rows, int64_t outs, int64_t cols, int dtype,
                                 void* weight_grad, void* bias_grad, void* workspace, optimi_stream_t stream_) {
   if (!valid_dtype(dtype)) return OPTIMI_ERR_DTYPE;
-  if (int rc = check_shape(rows, outs)) return rc;
-  if (int rc = check_shape(rows, cols)) return rc;
-  if (outs > kMostWidth || cols > kMostWidth) return OPTIMI_ERR_SIZE;
+  if (int rc = weight_grad_sizes(rows, outs, cols, dtype, bias_grad != nullptr)) return rc;
   if (outs == 0) return 0;
   if ((cols && !weight_grad) || (rows && (!grad || (cols && (!scales || !values))))) return OPTIMI_ERR_NULL;
   const int64_t size = elem_bytes(dtype);
@@ -1432,8 +1447,8 @@ int optimi_hip_int8_weight_grad(const void* grad, const int8_t* values, const fl
   if (c.tile == 256 && !direct) {
     c.tile = 128;
     c.tiles = tiles_of(outs, cols, 128);
+    if (!launch_holds(c.tiles * c.splits, kWeightGradLanes)) return OPTIMI_ERR_ALIGN;
   }
-  if (c.tiles * c.splits > kMostTiles) return OPTIMI_ERR_SIZE;
   return by_dtype(dtype, [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     const dim3 grid((unsigned)(c.tiles * c.splits));

@@ -671,6 +671,7 @@ int optimi_hip_add_rms_norm_int8(const void* x, const void* residual, const void
 
 int64_t optimi_hip_add_rms_norm_int8_backward_workspace(int64_t rows, int64_t cols) {
   if (int rc = check_shape(rows, cols)) return rc;
+  if (cols == 0) return OPTIMI_ERR_SIZE;
   return norm_partials(rows, cols) * cols * 4;
 }
 

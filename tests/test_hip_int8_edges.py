@@ -8,7 +8,7 @@ from torch import nn
 import int8_ref as R
 import optimi_amd as optimi
 from optimi_amd import backend
-from test_hip_int8 import checkpoint, norm_layers, rand
+from test_hip_int8 import checkpoint, int8_inputs, misaligned, norm_layers, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -201,3 +201,24 @@ def test_one_of_two_layers_is_trained(hip_device):
     values, scales, _, _ = optimi.add_rms_norm_int8(x.to(hip_device), ln)
     assert torch.equal(lw[0].grad, optimi.int8_weight_grad(gs[0], values, scales))
     R.close(lb.grad, *R.column_sum(gs[1].cpu(), torch.bfloat16), "bias")
+
+
+# ---------------------------------------------------------------------------------- the most outputs
+
+@pytest.mark.parametrize("m", [1, 4, 70])
+def test_products_of_very_many_outputs(hip_device, m):
+    """Launches of nearly 2^32 lanes and, off the 16-byte grid, of 2^23 tiles."""
+    n, k = (1 << 28) - 16 if m < 5 else 1 << 28, 16
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("needs 60 GB of device memory")
+    a, sa, _, _ = (t.to(hip_device) for t in int8_inputs(m, 1, k, 1))
+    b, sb = torch.zeros(n, k, dtype=torch.int8, device=hip_device), torch.ones(n, device=hip_device)
+    places = [slice(0, 300), slice((1 << 27) - 100, (1 << 27) + 200), slice(n - 300, n)]
+    for i, at in enumerate(places):
+        b[at] = torch.randint(-127, 128, (300, k), generator=torch.Generator().manual_seed(i), dtype=torch.int8).to(hip_device)
+    if m > 4:
+        b = misaligned(b, hip_device)
+    y = optimi.int8_matmul(a, sa, b, sb)
+    for at in places:
+        assert torch.equal(y[:, at], optimi.int8_matmul(a, sa, b[at], sb[at]))
+    assert not y[:, 300:1000].any() and not y[:, 1 << 26:(1 << 26) + 5000].any() and not y[:, n - 5000:n - 300].any()

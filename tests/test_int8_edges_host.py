@@ -1,11 +1,55 @@
 """What the int8 operators refuse and what a prepared model runs as before, at the edges; no GPU is touched."""
 
+import ctypes
+
 import pytest
 import torch
 from torch import nn
 
 import optimi_amd as optimi
-from optimi_amd import int8
+from optimi_amd import cabi, int8
+
+P = ctypes.c_void_p(256)  # never dereferenced: every call below is refused
+UNALIGNED = ctypes.c_void_p(264)
+
+
+# ---------------------------------------------------------------------------------- sizes
+
+@pytest.mark.parametrize("m,n,k", [(1 << 30, 1 << 28, 8), (1 << 30, 1 << 28, 7), (5, 4, 131072), (-1, 4, 8), (4, 1 << 29, 8), (1 << 31, 4, 8)])
+def test_matmul_and_its_workspace_refuse_the_same_sizes(m, n, k):
+    L = cabi.lib()
+    for dtype in (cabi.F32, cabi.BF16, cabi.F16):
+        assert L.optimi_hip_int8_matmul(P, P, P, P, None, m, n, k, dtype, P, P, None) == -2
+    assert L.optimi_hip_int8_matmul_workspace(m, n, k) == -2
+
+
+def test_the_widest_weight_is_taken_for_any_number_of_rows():
+    for m in (1, 4, 5, 64):
+        assert cabi.lib().optimi_hip_int8_matmul_workspace(m, 1 << 28, 16) == 0
+
+
+@pytest.mark.parametrize("rows,outs,cols", [(64, 1 << 24, 1 << 24), (8, (1 << 24) + 1, 4), (8, 4, (1 << 24) + 1), (1 << 31, 4, 4), (8, -1, 4), (8, 4, -1)])
+def test_weight_grad_and_its_workspace_refuse_the_same_sizes(rows, outs, cols):
+    L = cabi.lib()
+    for dtype in (cabi.F32, cabi.BF16, cabi.F16):
+        for bias in (None, P):
+            assert L.optimi_hip_int8_weight_grad(P, P, P, rows, outs, cols, dtype, P, bias, P, None) == -2
+            assert L.optimi_hip_int8_weight_grad_workspace(rows, outs, cols, dtype, bias is not None) == -2
+
+
+def test_the_norm_and_its_workspace_refuse_the_same_sizes():
+    L = cabi.lib()
+    for rows, cols in ((5, 0), (0, 0), (-1, 8), (5, -8), (1 << 31, 8), (5, 1 << 29)):
+        assert L.optimi_hip_add_rms_norm_int8_backward(P, None, P, P, P, rows, cols, cabi.BF16, cabi.BF16, P, P, P, None) == -2
+        assert L.optimi_hip_add_rms_norm_int8_backward_workspace(rows, cols) == -2
+
+
+def test_a_product_too_large_for_small_tiles_asks_for_alignment():
+    """Operands off the 16-byte grid go through 64 x 64 tiles; where a launch cannot hold so many, that is said."""
+    L = cabi.lib()
+    m, n, k = 1 << 20, 1 << 17, 64
+    assert L.optimi_hip_int8_matmul_workspace(m, n, k) == 0
+    assert L.optimi_hip_int8_matmul(UNALIGNED, P, P, P, None, m, n, k, cabi.BF16, P, None, None) == -4
 
 
 # ---------------------------------------------------------------------------------- which modules run as one node
