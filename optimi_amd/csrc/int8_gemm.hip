@@ -727,8 +727,8 @@ __device__ __forceinline__ u32x2 widen(uint32_t word, float s) {
   return u32x2{Product<DT>::pair(f[0], f[1]), Product<DT>::pair(f[2], f[3])};
 }
 
-// A wave's 16 kN x 16 kC sums, 16 rows at a time through LDS.
-template <int DT, class O, int kN, int kC>
+// A wave's 16 kN x 16 kC sums, 16 rows at a time through LDS: to the result or, with PARTS where the sum is split, to a part's place.
+template <int DT, class O, bool PARTS, int kN, int kC>
 __device__ __forceinline__ void store_sums(const WeightGradArgs& p, const f32x4 (&acc)[kN][kC], uint32_t* block, int split, int64_t n0, int64_t c0) {
   using T = typename Elem<DT>::type;
   const int lane = threadIdx.x % 64;
@@ -746,7 +746,7 @@ __device__ __forceinline__ void store_sums(const WeightGradArgs& p, const f32x4 
       O::get(block, O::row(t), v);
       const float(&f)[8] = reinterpret_cast<const float(&)[8]>(v);
       if (n < p.outs && some > 0) {
-        if (p.splits > 1) store_some<OPTIMI_F32>(p.partial + ((int64_t)split * p.outs + n) * p.cols + c, f, some);
+        if (PARTS && p.splits > 1) store_some<OPTIMI_F32>(p.partial + ((int64_t)split * p.outs + n) * p.cols + c, f, some);
         else store_some<DT>((T*)p.out + n * p.cols + c, f, some, whole_lines(p.cols, sizeof(T)));
       }
     }
@@ -949,14 +949,14 @@ __global__ void __launch_bounds__(512) weight_grad_kernel(WeightGradArgs p) {
 
   using O = OutBlock<16, 32>;
   static_assert(kWaves / 2 * O::kBytes <= kPlane * 2, "half of the waves' blocks fit a tile");
-  store_sums<DT, O, kN, kC>(p, acc, (uint32_t*)((char*)(wave < 4 ? g1 : q1) + wave % 4 * O::kBytes), split, n0 + wn, c0 + wc);
+  store_sums<DT, O, true, kN, kC>(p, acc, (uint32_t*)((char*)(wave < 4 ? g1 : q1) + wave % 4 * O::kBytes), split, n0 + wn, c0 + wc);
 }
 
 // The same for large 16-bit products, where all that counts is that the matrix instructions never wait: 256 x 256 tiles, 64
 // rows a step, two pairs of tiles in LDS, eight wavefronts with 128 x 64 sums each.  Gradients go to LDS past the registers;
 // the values have to become 16-bit numbers on the way, and are loaded two steps ahead, so that the conversion of the next
 // step's values can be spread over this step's products without waiting for memory.  outs is a multiple of 8, grad aligned to
-// 16 bytes, and a row has 16 values at least.
+// 16 bytes, a row has 16 values at least, and there are more than 128 tiles: their sums are never split.
 //
 // 8192 x 11008 x 4096 bf16: 676 us, 1.09 PFLOP/s (a library's bf16 product of these operands in this layout, the values widened
 // beforehand: 0.89); a step takes 3900 busy cycles by the counters, of which the matrix units are busy for 2048, LDS for 1300 (a
@@ -970,13 +970,11 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
   using H = HalfTile<kTile>;
   __shared__ __attribute__((aligned(1024))) short g0[kRows * kTile], g1[kRows * kTile], q0[kRows * kTile], q1[kRows * kTile];
   const int tn = (int)((p.outs + kTile - 1) / kTile), tc = (int)((p.cols + kTile - 1) / kTile);
-  const int split = blockIdx.x / (tn * tc);
-  const Tile tile = tile_of(blockIdx.x % (tn * tc), tn, tc);
+  const Tile tile = tile_of(blockIdx.x, tn, tc);
   const int64_t n0 = (int64_t)tile.row * kTile, c0 = (int64_t)tile.col * kTile;
   const int wave = wave_id(), lane = threadIdx.x % 64;
   const int wn = wave / 4 * 128, wc = wave % 4 * 64;
   const int all = (int)((p.rows + kRows - 1) / kRows);
-  const int begin = split * p.steps_per_split, end = begin + p.steps_per_split < all ? begin + p.steps_per_split : all;
 
   f32x4 acc[kN][kC];
 #pragma unroll
@@ -1074,7 +1072,6 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
     return v & 0x7fff;
   };
   const int first_g = (H::at(lane / 4, wn / 16) + lane % 4 * 4) * 2, first_q = (H::at(lane / 4, wc / 16) + lane % 4 * 4) * 2;
-  const int left = end == all ? (int)(p.rows - (int64_t)(all - 1) * kRows) : kRows;
   // One step's products in sixteen groups; a group's operands are read two groups earlier, and four of the groups are followed
   // by a quarter of the next step's conversion.
   auto multiply = [&](const short* g, const short* q, auto last, const u32x4 (&v)[kPieces], const float (&s)[kPieces], short* next) OPTIMI_INLINE {
@@ -1084,7 +1081,7 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
       if (!last.value) return f;
       s16x8 mask;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) mask[e] = ks * 32 + e / 4 * 16 + lane / 16 * 4 + e % 4 < left ? -1 : 0;
+      for (int e = 0; e < 8; ++e) mask[e] = ks * 32 + e / 4 * 16 + lane / 16 * 4 + e % 4 < last_rows ? -1 : 0;
       return f & mask;
     };
 #pragma unroll
@@ -1109,7 +1106,7 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
   auto step_on = [&](int step, auto which) OPTIMI_INLINE {
     constexpr int W = decltype(which)::value;
     copy(step + 1, W ? g0 : g1);
-    if (step + 2 < end) load(step + 2, vq[W], sq[W]);
+    if (step + 2 < all) load(step + 2, vq[W], sq[W]);
     if (step + 2 == all) shift(step + 1, vq[1 - W], sq[1 - W]);
     __builtin_amdgcn_sched_barrier(0);  // the loads start before the products do; left alone, they are moved behind them
     multiply(W ? g1 : g0, W ? q1 : q0, std::false_type{}, vq[1 - W], sq[1 - W], W ? q0 : q1);
@@ -1119,7 +1116,7 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
     constexpr int W = decltype(which)::value;
     copy(step, W ? g1 : g0);
     load(step, vq[W], sq[W]);
-    if (step + 1 < end) load(step + 1, vq[1 - W], sq[1 - W]);
+    if (step + 1 < all) load(step + 1, vq[1 - W], sq[1 - W]);
     if (step + 1 == all) shift(step, vq[W], sq[W]);
 #pragma unroll
     for (int half = 0; half < 2 * kPieces; ++half) write_half(half, vq[W], sq[W], W ? q1 : q0);
@@ -1127,23 +1124,21 @@ __global__ void __launch_bounds__(512) weight_grad_wide_kernel(WeightGradArgs p)
   };
 
   // the last step works on the first pair of tiles
-  if (begin < end) {
-    int step = begin;
-    if ((end - begin) % 2) {
-      start(step, Pair<0>{});
-    } else {
-      start(step, Pair<1>{});
-      step_on(step++, Pair<1>{});
-    }
-    for (; step + 1 < end; step += 2) {
-      step_on(step, Pair<0>{});
-      step_on(step + 1, Pair<1>{});
-    }
-    multiply(g0, q0, std::true_type{}, vq[0], sq[0], q1);
+  int step = 0;
+  if (all % 2) {
+    start(step, Pair<0>{});
+  } else {
+    start(step, Pair<1>{});
+    step_on(step++, Pair<1>{});
   }
+  for (; step + 1 < all; step += 2) {
+    step_on(step, Pair<0>{});
+    step_on(step + 1, Pair<1>{});
+  }
+  multiply(g0, q0, std::true_type{}, vq[0], sq[0], q1);
 
   using O = OutBlock<16, 64>;
-  store_sums<DT, O, kN, kC>(p, acc, (uint32_t*)((char*)(wave < 4 ? g1 : q1) + wave % 4 * O::kBytes), split, n0 + wn, c0 + wc);
+  store_sums<DT, O, false, kN, kC>(p, acc, (uint32_t*)((char*)(wave < 4 ? g1 : q1) + wave % 4 * O::kBytes), 0, n0 + wn, c0 + wc);
 }
 
 // Adds the splits' sums, four neighbours a lane, always in the same order.
@@ -1243,10 +1238,10 @@ Cut weight_grad_cut(int64_t rows, int64_t outs, int64_t cols, int dtype) {
   const double c256 = 2.2 * (double)((t256 + kCus - 1) / kCus);
   const double c128 = t128 <= kCus ? 0.8 : 1.45 * (double)((t128 + 2 * kCus - 1) / (2 * kCus));
   const bool wide = dtype != OPTIMI_F32 && !narrow && rows * cols >= 16;
-  c.tile = wide && t256 >= kCus / 2 && c256 <= c128 ? 256 : 128;
+  c.tile = wide && c256 <= c128 ? 256 : 128;  // 129 wide tiles at least: where that holds, t128 is above 512
   c.tiles = tiles_of(outs, cols, c.tile);
   int64_t parts = 1;
-  if (c.tiles < kCus) parts = kCus / c.tiles < steps / 4 ? kCus / c.tiles : steps / 4;
+  if (c.tile == 128 && c.tiles < kCus) parts = kCus / c.tiles < steps / 4 ? kCus / c.tiles : steps / 4;
   c.split(steps, parts < 16 ? parts : 16);
   return c;
 }
