@@ -8,7 +8,7 @@ from torch import nn
 import int8_ref as R
 import optimi_amd as optimi
 from optimi_amd import backend
-from test_hip_int8 import checkpoint, int8_inputs, misaligned, norm_layers, rand
+from test_hip_int8 import Guarded, checkpoint, int8_inputs, misaligned, norm_layers, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -201,6 +201,63 @@ def test_one_of_two_layers_is_trained(hip_device):
     values, scales, _, _ = optimi.add_rms_norm_int8(x.to(hip_device), ln)
     assert torch.equal(lw[0].grad, optimi.int8_weight_grad(gs[0], values, scales))
     R.close(lb.grad, *R.column_sum(gs[1].cpu(), torch.bfloat16), "bias")
+
+
+# ---------------------------------------------------------------------------------- bias gradients of large layers
+
+# the wide kernel's sizes (in 16 bits): the bias gradient is a sum of columns beside it, one to three stripes of 2048
+# columns, with and without a padded copy in front of its workspace, rows above and below the 128 partial sums
+WIDE = [(1, 3000, 2900), (65, 3000, 2800), (127, 2904, 2831), (129, 2817, 3000), (200, 2896, 2817), (257, 5000, 1700), (1000, 2817, 2820), (300, 1000, 8300)]
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES, ids=R.IDS)
+@pytest.mark.parametrize("shape", WIDE, ids=lambda s: "x".join(map(str, s)))
+def test_bias_gradient_of_large_layers(hip_device, shape, dtype):
+    rows, outs, cols = shape
+    g, (q, s) = rand((rows, outs), dtype, 3, 1e-2).to(hip_device), (t.to(hip_device) for t in checkpoint(rows, cols, 4))
+    want, allowed = R.weight_grad(g, q, s, dtype)
+    bias, bias_allowed = R.column_sum(g.cpu(), dtype)
+    for grad, values in ((g, q), (misaligned(g, hip_device), misaligned(q, hip_device))):
+        dw, db = optimi.int8_weight_grad(grad, values, s, bias=True)
+        R.close(dw, want.cpu(), allowed.cpu(), f"weight {shape}")
+        R.close(db, bias, bias_allowed, f"bias {shape}")
+        again = optimi.int8_weight_grad(grad, values, s, bias=True)
+        assert torch.equal(again[0], dw) and torch.equal(again[1], db), "the same bits on every run"
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES, ids=R.IDS)
+@pytest.mark.parametrize("shape", [(65, 3000, 2800), (130, 2904, 2831), (129, 2817, 3000)], ids=lambda s: "x".join(map(str, s)))
+def test_bias_gradient_of_large_layers_that_is_not_finite(hip_device, shape, dtype):
+    rows, outs, cols = shape
+    g, (q, s) = rand((rows, outs), dtype, 4, 1e-2).to(hip_device), (t.to(hip_device) for t in checkpoint(rows, cols, 5))
+    g[rows - 1, 5], g[0, 9], g[rows // 2, outs - 1] = float("inf"), float("-inf"), float("nan")
+    _, db = optimi.int8_weight_grad(g, q, s, bias=True)
+    R.close(db, *R.column_sum(g.cpu(), dtype), "bias")
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES, ids=R.IDS)
+@pytest.mark.parametrize("shape", [(129, 2817, 3000), (257, 5000, 1700)], ids=lambda s: "x".join(map(str, s)))
+def test_a_large_weight_gradient_stays_in_its_buffers(hip_device, shape, dtype):
+    """Through the C ABI, into buffers and a workspace of exactly the stated size with margins around them."""
+    from optimi_amd import cabi
+    L, code = cabi.lib(), {torch.float32: cabi.F32, torch.bfloat16: cabi.BF16, torch.float16: cabi.F16}[dtype]
+    rows, outs, cols = shape
+    g, (q, s) = rand((rows, outs), dtype, 3, 1e-2), checkpoint(rows, cols, 4)
+    want, allowed = R.weight_grad(*(t.to(hip_device) for t in (g, q, s)), dtype)
+    for offset in (0, 1):
+        buf = Guarded(hip_device)
+        dg, dq, ds = (buf(t, offset=offset) for t in (g, q, s))
+        dw, db = buf(shape=(outs, cols), dtype=dtype, offset=offset), buf(shape=(outs,), dtype=dtype, offset=offset)
+        size = L.optimi_hip_int8_weight_grad_workspace(rows, outs, cols, code, 1)
+        assert size >= 0
+        work = buf(shape=(size,), dtype=torch.uint8) if size else None
+        pointers = [t.data_ptr() for t in (dg, dq, ds)], [t.data_ptr() for t in (dw, db)]
+        cabi.check(L.optimi_hip_int8_weight_grad(*pointers[0], rows, outs, cols, code, *pointers[1], None if work is None else work.data_ptr(),
+                                                 torch.cuda.current_stream().cuda_stream), "weight_grad")
+        torch.cuda.synchronize()
+        buf.check()
+        R.close(dw, want.cpu(), allowed.cpu(), "weight")
+        R.close(db, *R.column_sum(g, dtype), "bias")
 
 
 # ---------------------------------------------------------------------------------- the most outputs
