@@ -106,3 +106,24 @@ def close(got, want, allowed, what=""):
         at = int(((got - want).abs() / allowed.clamp(min=1e-300)).where(~special, torch.zeros_like(got)).flatten().argmax())
         raise AssertionError(f"{what}: {int(over.sum())} of {over.numel()} off, worst at {at}: got {got.flatten()[at]}, "
                              f"want {want.flatten()[at]}, allowed {allowed.flatten()[at]}")
+
+
+# Rows that end inside a vector of eight: the kernels read the row's last eight elements there, some of which are the
+# neighbour's too.
+RAGGED = [9, 13, 65, 511, 513, 1023, 1025, 2047, 2049, 4097, 6145, 8193, 12289, 16385, 18001, 20003]
+
+
+def loud_places(cols):
+    """Columns to put a loud element at: first and last of those that two vectors share, before them, and the row's last."""
+    shared = range(cols - 8, cols - cols % 8)
+    return sorted({shared[0], shared[-1], max(0, shared[0] - 1), cols - 1})
+
+
+def loud_row(cols, at, dtype, wdtype):
+    """(h, g, w): three rows of small numbers with one large one in column `at` of the activation and of its gradient."""
+    gen = torch.Generator().manual_seed(cols + at)
+    h = torch.randn(3, cols, generator=gen, dtype=torch.float64) * 2.0**-9
+    g = torch.randn(3, cols, generator=gen, dtype=torch.float64) * 2.0**-9
+    h[:, at], g[:, at] = 24.0, 4.0
+    w = 1 + 0.2 * torch.rand(cols, generator=gen, dtype=torch.float64)
+    return h.to(dtype), g.to(dtype), w.to(wdtype)

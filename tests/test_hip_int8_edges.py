@@ -260,6 +260,28 @@ def test_a_large_weight_gradient_stays_in_its_buffers(hip_device, shape, dtype):
         R.close(db, *R.column_sum(g, dtype), "bias")
 
 
+# ---------------------------------------------------------------------------------- rows that end inside a vector
+
+@pytest.mark.parametrize("weight32", [False, True], ids=["weight_own", "weight_fp32"])
+@pytest.mark.parametrize("dtype", R.DTYPES, ids=R.IDS)
+@pytest.mark.parametrize("cols", R.RAGGED)
+def test_every_element_counts_once(hip_device, cols, dtype, weight32):
+    """One loud element in the columns that the last vector shares with its neighbour, or beside them: counted twice or not at
+    all, it changes everything by a factor (the oracle with that mistake is held against the allowances on the CPU)."""
+    for at in R.loud_places(cols):
+        h, g, w = R.loud_row(cols, at, dtype, torch.float32 if weight32 else dtype)
+        values, scales, _, rstd = optimi.add_rms_norm_int8(h.to(hip_device), w.to(hip_device), eps=1e-6)
+        y, r, rel_r, rel_y = R.norm(h, w, 1e-6)
+        R.close(rstd, r, rel_r * r, f"rstd {at}")
+        s = scales.cpu().double()[:, None]
+        R.close(values.cpu().double() * s, y, s / 2 + rel_y * y.abs(), f"y {at}")
+        r = r.float()
+        dx, dw = optimi.add_rms_norm_int8_backward(g.to(hip_device), h.to(hip_device), r.to(hip_device), w.to(hip_device))
+        want_dx, allow_dx, want_dw, allow_dw = R.norm_backward(g, h, r, w, None, dtype, w.dtype)
+        R.close(dx, want_dx, allow_dx, f"dx {at}")
+        R.close(dw, want_dw, allow_dw, f"dweight {at}")
+
+
 # ---------------------------------------------------------------------------------- the most outputs
 
 @pytest.mark.parametrize("m", [1, 4, 70])
