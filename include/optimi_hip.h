@@ -387,8 +387,8 @@ int optimi_hip_int8_weight_grad(const void* grad, const int8_t* values, const fl
                                 optimi_stream_t stream);
 
 /* h = x + residual (rounded to `dtype`; x itself, and h not written, where residual is NULL),
- * rstd[r] = 1 / sqrt(mean(h[r]^2) + eps), and the int8 form of y[r][c] = h[r][c] * rstd[r] * weight[c], which is
- * formed in fp32 and not rounded before.  weight is of `weight_dtype`: `dtype` or OPTIMI_F32.  cols >= 1. */
+ * rstd[r] = 1 / sqrt(mean(h[r]^2) + eps), also where squares leave fp32's range, and the int8 form of
+ * y[r][c] = h[r][c] * rstd[r] * weight[c], which is formed in fp32 and not rounded before.  weight is of `weight_dtype`: `dtype` or OPTIMI_F32.  cols >= 1. */
 int optimi_hip_add_rms_norm_int8(const void* x, const void* residual, const void* weight, int64_t rows, int64_t cols,
                                  int dtype, int weight_dtype, double eps, void* h, int8_t* values, float* scales, float* rstd,
                                  optimi_stream_t stream);

@@ -203,6 +203,94 @@ def test_one_of_two_layers_is_trained(hip_device):
     R.close(lb.grad, *R.column_sum(gs[1].cpu(), torch.bfloat16), "bias")
 
 
+# ---------------------------------------------------------------------------------- rows whose squares leave float32's range
+
+ROW_WIDTHS = [1, 5, 8, 100, 513, 1001, 1500, 4100, 6000, 8200, 9000, 13000, 16385, 18001]
+
+
+def extreme_rows(cols, dtype, sizes, seed):
+    gen = torch.Generator().manual_seed(seed)
+    x = (1 + torch.rand(len(sizes), cols, generator=gen, dtype=torch.float64)) * torch.where(torch.rand(len(sizes), cols, generator=gen) < 0.5, -1, 1)
+    return (x * torch.tensor(sizes, dtype=torch.float64)[:, None]).to(dtype)
+
+
+def check_extreme_norm(device, x, w, eps, residual=None):
+    h = x if residual is None else (x.double() + residual.double()).to(x.dtype)
+    values, scales, _, rstd = optimi.add_rms_norm_int8(x.to(device), w.to(device), residual=None if residual is None else residual.to(device), eps=eps)
+    y, r, rel_r, rel_y = R.norm(h, w, eps)
+    # 1/rms of the largest rows is below float32's normal range: two roundings to its smallest step
+    coarse = 2.02 * R.least(torch.float32)
+    R.close(rstd, r, rel_r * r + coarse, "rstd")
+    q, s = values.cpu().double(), scales.cpu().double()
+    assert bool((q.abs() <= 127).all())
+    absmax = y.abs().amax(1, keepdim=True)
+    assert bool((s[:, None] <= 2 * absmax / 63).all()), "a scale that does not fit its row"
+    R.close(q * s[:, None], y, s[:, None] / 2 + (rel_y + coarse / r[:, None]) * y.abs(), "y")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("cols", ROW_WIDTHS)
+def test_norm_of_large_rows(hip_device, cols, dtype):
+    """Finite rows whose squares have no place in float32 have an ordinary norm."""
+    sizes = [2.0**e for e in (50, 57, 60, 63, 64, 80, 100, 120, 126)] + [1.0]
+    x = extreme_rows(cols, dtype, sizes, cols)
+    w = (1 + 0.2 * torch.rand(cols, generator=torch.Generator().manual_seed(1), dtype=torch.float64)).to(dtype)
+    check_extreme_norm(hip_device, x, w, 1e-6)
+    check_extreme_norm(hip_device, x / 2, w, 1e-6, residual=(x / 4).flip(0).contiguous())
+
+
+@pytest.mark.parametrize("eps", [0.0, 1e-50, 1e-38, 1e-30])
+@pytest.mark.parametrize("dtype", R.DTYPES, ids=R.IDS)
+@pytest.mark.parametrize("cols", ROW_WIDTHS)
+def test_norm_of_small_rows(hip_device, cols, dtype, eps):
+    """With an eps below it, a row of tiny numbers has a norm as good as another's."""
+    low = -22 if dtype == torch.float16 else -100
+    x = extreme_rows(cols, dtype, [2.0**e for e in (low, low / 2, -20, -1)], cols + 1)
+    if dtype != torch.float16:  # numbers of unlike size, the small ones below the range of squares altogether
+        x = torch.cat([x, extreme_rows(cols, dtype, [2.0**-40, 2.0**-55, 2.0**-60, 2.0**-75], cols + 2)])
+        x[-1, : cols // 2] *= 2.0**-40
+    w = (1 + 0.2 * torch.rand(cols, generator=torch.Generator().manual_seed(1), dtype=torch.float64)).to(dtype)
+    check_extreme_norm(hip_device, x, w, eps)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("cols", [3, 40, 1500, 17000])
+def test_norm_of_rows_whose_inverse_rms_is_too_large(hip_device, cols, dtype):
+    """Subnormal rows without an eps: 1/rms has no place in float32, the normed row has."""
+    x = extreme_rows(cols, dtype, [2.0**-130, 2.0**-131], cols)
+    values, scales, _, rstd = optimi.add_rms_norm_int8(x.to(hip_device), torch.ones(cols, dtype=dtype, device=hip_device), eps=0.0)
+    y, _, _, rel_y = R.norm(x, torch.ones(cols), 0.0)
+    s = scales.cpu().double()[:, None]
+    R.close(values.cpu().double() * s, y, s / 2 + rel_y * y.abs(), "y")
+    assert bool(torch.isinf(rstd).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("cols", [1, 40, 1500, 4100, 9000, 17000])
+def test_norm_backward_of_extreme_rows(hip_device, cols, dtype):
+    sizes = [2.0**e for e in (-100, -80, -64, -50, 50, 64, 80, 100, 126)]
+    h, w = extreme_rows(cols, dtype, sizes, cols), torch.ones(cols, dtype=dtype)
+    g, gh = rand((len(sizes), cols), dtype, 2, 1e-2), rand((len(sizes), cols), dtype, 3, 1e-2)
+    rstd = R.norm(h, w, 0.0)[1].float()
+    for more in (None, gh):
+        dx, dw = optimi.add_rms_norm_int8_backward(*(t.to(hip_device) for t in (g, h, rstd, w)), grad_h=None if more is None else more.to(hip_device))
+        want_dx, allow_dx, want_dw, allow_dw = R.norm_backward(g, h, rstd, w, more, dtype, dtype)
+        R.close(dx, want_dx, allow_dx, "dx")
+        R.close(dw, want_dw, allow_dw, "dweight")
+
+
+@pytest.mark.parametrize("cols", [40, 1500, 17000])
+def test_norm_of_extreme_rows_that_are_empty_or_not_finite(hip_device, cols):
+    x = extreme_rows(cols, torch.bfloat16, [2.0**100] * 4, 1)
+    x[0], x[1, 3], x[2, 5] = 0, float("inf"), float("nan")
+    w = torch.ones(cols, dtype=torch.bfloat16)
+    for eps in (1e-6, 1e-50):
+        values, scales, _, rstd = (t.cpu() for t in optimi.add_rms_norm_int8(x.to(hip_device), w.to(hip_device), eps=eps))
+        assert torch.equal(torch.isnan(scales), torch.tensor([False, True, True, False]))
+        assert float(scales[0]) == 1.0 and not values[:3].any() and bool(values[3].any())
+        assert abs(float(rstd[0]) * eps**0.5 - 1) < 4 * R.U
+
+
 # ---------------------------------------------------------------------------------- bias gradients of large layers
 
 # the wide kernel's sizes (in 16 bits): the bias gradient is a sum of columns beside it, one to three stripes of 2048
