@@ -272,6 +272,12 @@ struct ByteTile {
   static __device__ __forceinline__ i32x4 read(const int8_t* lds, int r, int c) { return *(const i32x4*)(lds + r * kStep + ((c ^ (r / 2 & 7)) * 16)); }
 };
 
+// v sa sb + bias.  A sum times a scale from 2^96 on can leave fp32's range where the result does not: the other scale goes first then.
+__device__ __forceinline__ bool goes_first(float scale) { return fabsf(scale) < 0x1p96f; }
+__device__ __forceinline__ float scaled(int32_t v, float sa, float sb, float bias) {
+  return goes_first(sa) ? fmaf((float)v * sa, sb, bias) : fmaf((float)v * sb, sa, bias);
+}
+
 // What every tile of the product shares: where it lies, one step's products, and the way out.
 template <int DT, int BM, int BN, int WM, int WN>
 struct MatmulTile {
@@ -357,23 +363,38 @@ struct MatmulTile {
           O::put(block, lane % 32, j * 8 + q * 2 + lane / 32, v);
         }
       __builtin_amdgcn_wave_barrier();
+      float sa[O::kTurns];
+      bool ordinary = true;
 #pragma unroll
       for (int t = 0; t < O::kTurns; ++t) {
         const int64_t m = m0 + wm + i * 32 + O::row(t);
-        uint32_t v[8];
-        O::get(block, O::row(t), v);
-        if (m < p.m && some > 0) {
-          if (p.splits > 1) {
-            store_some<OPTIMI_F32>((float*)p.partial + ((int64_t)split * p.m + m) * p.n + n, reinterpret_cast<const float(&)[8]>(v), some);
-          } else {
-            const float sa = p.a_scales[m];
-            float f[8];
+        sa[t] = p.splits == 1 ? p.a_scales[m < p.m ? m : p.m - 1] : 0.0f;
+        ordinary &= goes_first(sa[t]);
+      }
+      // a branch for all of a lane's rows instead of a choice for each number
+      auto rows = [&](auto any) OPTIMI_INLINE {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = fmaf((float)(int32_t)v[e] * sa, sb[e], bias[e]);
-            store_some<DT>((T*)p.out + m * p.n + n, f, some, whole_lines(p.n, sizeof(T)));
+        for (int t = 0; t < O::kTurns; ++t) {
+          const int64_t m = m0 + wm + i * 32 + O::row(t);
+          uint32_t v[8];
+          O::get(block, O::row(t), v);
+          if (m < p.m && some > 0) {
+            if (p.splits > 1) {
+              store_some<OPTIMI_F32>((float*)p.partial + ((int64_t)split * p.m + m) * p.n + n, reinterpret_cast<const float(&)[8]>(v), some);
+            } else {
+              float f[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                if (any.value) f[e] = scaled((int32_t)v[e], sa[t], sb[e], bias[e]);
+                else f[e] = fmaf((float)(int32_t)v[e] * sa[t], sb[e], bias[e]);
+              }
+              store_some<DT>((T*)p.out + m * p.n + n, f, some, whole_lines(p.n, sizeof(T)));
+            }
           }
         }
-      }
+      };
+      if (ordinary) rows(std::false_type{});
+      else rows(std::true_type{});
       __builtin_amdgcn_wave_barrier();
     }
   }
@@ -582,7 +603,7 @@ __global__ void __launch_bounds__(256) matvec_kernel(MatmulArgs p) {
   const int64_t m = lane % M, n = n0 + lane / M;
   if (m >= p.m || n >= p.n) return;
   const float bias = p.bias ? E::get(((const T*)p.bias)[n]) : 0.0f;
-  ((T*)p.out)[m * p.n + n] = E::put(fmaf((float)sum * p.a_scales[m], p.b_scales[n], bias));
+  ((T*)p.out)[m * p.n + n] = E::put(scaled(sum, p.a_scales[m], p.b_scales[n], bias));
 }
 
 // Copies of up to two matrices whose rows of `from` bytes lie `to` bytes apart afterwards, a multiple of 16, with zeros in between: what
@@ -629,7 +650,7 @@ __global__ void __launch_bounds__(256) matmul_finish_kernel(MatmulArgs p) {
     for (int e = 0; e < 4; ++e) {
       if (e >= some) break;
       const float bias = p.bias ? E::get(((const T*)p.bias)[n]) : 0.0f;
-      ((T*)p.out)[at + e] = E::put(fmaf((float)sum[e] * p.a_scales[m], p.b_scales[n], bias));
+      ((T*)p.out)[at + e] = E::put(scaled(sum[e], p.a_scales[m], p.b_scales[n], bias));
       if (++n == p.n) {
         n = 0;
         ++m;

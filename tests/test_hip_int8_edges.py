@@ -291,6 +291,26 @@ def test_norm_of_extreme_rows_that_are_empty_or_not_finite(hip_device, cols):
         assert abs(float(rstd[0]) * eps**0.5 - 1) < 4 * R.U
 
 
+# ---------------------------------------------------------------------------------- scales at the ends of the range
+
+@pytest.mark.parametrize("shape", [(1, 100, 2000), (4, 40, 64), (40, 70, 96), (100, 100, 16384), (130, 300, 1111), (2600, 2700, 131), (4096, 4096, 64)], ids=lambda s: "x".join(map(str, s)))
+def test_matmul_of_scales_whose_product_is_ordinary(hip_device, shape):
+    """A row of huge numbers against small weights, and the other way round: only the result has to fit the type."""
+    m, n, k = shape
+    a, _, b, _ = int8_inputs(m, n, k, 5)
+    bias = rand((n,), torch.float32, 6)
+    big, small = torch.full((m,), 2.0**110), torch.full((n,), 2.0**-115)
+    big[m // 2] = 2.0**121
+    small[n // 2] = 2.0**-126
+    for sa, sb in ((big, small), (torch.full((m,), 2.0**-126), torch.full((n,), 2.0**121))):
+        y = optimi.int8_matmul(a.to(hip_device), sa.to(hip_device), b.to(hip_device), sb.to(hip_device), bias=bias.to(hip_device), dtype=torch.float32)
+        if m * n * k < 1 << 29:
+            want, allowed = R.matmul(a, sa, b, sb, bias, torch.float32)
+        else:
+            want, allowed = (t.cpu() for t in R.matmul(*(t.to(hip_device) for t in (a, sa, b, sb, bias)), torch.float32))
+        R.close(y, want, allowed, str(shape))
+
+
 # ---------------------------------------------------------------------------------- bias gradients of large layers
 
 # the wide kernel's sizes (in 16 bits): the bias gradient is a sum of columns beside it, one to three stripes of 2048
