@@ -245,13 +245,14 @@ class _Int8Sequential(nn.Sequential):
 
 _PREPARED = {nn.Linear: Int8Linear, nn.Sequential: _Int8Sequential}
 _MODULES_ATTR = "_int8_linear_modules"
+_MOST_INPUTS = 131071  # that a sum of int8 products in 32 bits holds
 
 
 def prepare_for_int8_linear(model: nn.Module, skip: Iterable[str] = ()) -> nn.Module:
     """Makes every ``nn.Linear`` of ``model`` (in place; itself included) an ``Int8Linear``, except those whose qualified
     name contains one of the strings in ``skip``, and lets an ``nn.RMSNorm`` directly before one in an ``nn.Sequential``
     hand it int8 values (under ``torch.autocast`` the norm takes its input as it comes, the layer runs in the autocast type).  Subclasses
-    of these modules are left alone.  Parameters stay the same objects: optimizers
+    of these modules and layers of more than 131071 inputs are left alone.  Parameters stay the same objects: optimizers
     built before or after, gradient release and checkpoints work as they did.  ``ValueError`` if the model is prepared
     already or holds no such layer.  Undo with ``remove_int8_linear``."""
     if isinstance(skip, str):
@@ -259,7 +260,8 @@ def prepare_for_int8_linear(model: nn.Module, skip: Iterable[str] = ()) -> nn.Mo
     skip = tuple(skip)
     if hasattr(model, _MODULES_ATTR):
         raise ValueError("`model` is prepared for int8 linear layers already.")
-    layers = [m for name, m in model.named_modules() if type(m) is nn.Linear and not any(s in name for s in skip)]
+    layers = [m for name, m in model.named_modules()
+              if type(m) is nn.Linear and m.in_features <= _MOST_INPUTS and not any(s in name for s in skip)]
     if not layers:
         raise ValueError("`model` has no `nn.Linear` to compute in int8.")
     changed = layers + [m for m in model.modules() if type(m) is nn.Sequential]

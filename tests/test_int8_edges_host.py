@@ -143,3 +143,17 @@ def test_hooks_on_all_modules_see_every_module(ran, register):
     assert "RMSNorm" in seen and "Int8Linear" in seen and ran == ["linear"]
     model(torch.randn(3, 8))
     assert ran == ["linear", "fused"]
+
+
+# ---------------------------------------------------------------------------------- layers that the product cannot take
+
+def test_preparation_leaves_layers_alone_that_are_too_wide():
+    """The product's sums hold 131071 inputs; a layer of more goes on as it was."""
+    with torch.device("meta"):
+        model = nn.Sequential(nn.RMSNorm(131072), nn.Linear(131072, 2), nn.Linear(2, 131072), nn.Linear(131071, 2))
+    optimi.prepare_for_int8_linear(model)
+    assert [type(m) for m in model] == [nn.RMSNorm, nn.Linear, optimi.Int8Linear, optimi.Int8Linear]
+    with torch.device("meta"):
+        wide = nn.Sequential(nn.Linear(131072, 2))
+    with pytest.raises(ValueError, match="no `nn.Linear`"):
+        optimi.prepare_for_int8_linear(wide)
