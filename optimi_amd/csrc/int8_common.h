@@ -279,6 +279,16 @@ __device__ __forceinline__ u32x2 quantize8(const float (&f)[8], const RowScale& 
 
 __device__ __forceinline__ uint32_t abs_bits(float f) { return __float_as_uint(f) & 0x7fffffffu; }
 
+// Calls f with the dtype code as a type, for a code that was checked.
+template <class F>
+int by_dtype(int dtype, F f) {
+  switch (dtype) {
+    case OPTIMI_F32: return f(std::integral_constant<int, OPTIMI_F32>{});
+    case OPTIMI_BF16: return f(std::integral_constant<int, OPTIMI_BF16>{});
+    default: return f(std::integral_constant<int, OPTIMI_F16>{});
+  }
+}
+
 // Grids are sized for rows below 2^31 and widths up to 2^28.
 inline int check_shape(int64_t rows, int64_t cols) {
   return rows < 0 || cols < 0 || rows >= ((int64_t)1 << 31) || cols > ((int64_t)1 << 28) ? (int)OPTIMI_ERR_SIZE : 0;

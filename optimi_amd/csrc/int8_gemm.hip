@@ -403,7 +403,7 @@ struct MatmulTile {
 // Rows that start on 16 bytes: two pairs of tiles in LDS, 256 x 256 (eight waves with 128 x 64 sums each, one workgroup a CU) or
 // 128 x 128 (four waves with 64 x 64, two workgroups a CU).  A step of 256 x 256 tiles is 64 KiB of copies for 2048 cycles of
 // matrix instructions on each SIMD; between two barriers nothing waits but for LDS, whose reads run one slice ahead.
-// 8192 x 11008 x 4096: 343 us, 2.15 Pop/s; the matrix units are busy for 61 % of the cycles at 1.95 GHz, and the 1376 tiles fill
+// 8192 x 11008 x 4096: 330 to 345 us from box to box, 2.14 to 2.24 Pop/s; the matrix units are busy for 61 % of the cycles at 1.95 GHz, and the 1376 tiles fill
 // 5.4 of 6 rounds.
 template <int DT, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(WM * WN * 64) matmul_kernel(MatmulArgs p) {
@@ -979,8 +979,8 @@ __global__ void __launch_bounds__(512) weight_grad_kernel(WeightGradArgs p) {
 // step's values can be spread over this step's products without waiting for memory.  outs is a multiple of 8, grad aligned to
 // 16 bytes, a row has 16 values at least, and there are more than 128 tiles: their sums are never split.
 //
-// 8192 x 11008 x 4096 bf16: 676 us, 1.09 PFLOP/s (a library's bf16 product of these operands in this layout, the values widened
-// beforehand: 0.89); a step takes 3900 busy cycles by the counters, of which the matrix units are busy for 2048, LDS for 1300 (a
+// 8192 x 11008 x 4096 bf16: 672 us among passes over changing inputs, 1.10 PFLOP/s; on one set of inputs in a row 648 us, where a library's
+// bf16 product of the same gradients and of the values widened beforehand takes 760; a step takes 3900 busy cycles by the counters, of which the matrix units are busy for 2048, LDS for 1300 (a
 // fifth of them bank conflicts) and vector instructions for 1000, two thirds of them the conversion: ten for four values (with eleven, and
 // the last step's borders worked out in every step, 735 us); 688 tiles fill 2.7 of 3 rounds.  A raised wave priority around the products changes nothing.
 template <int DT>
@@ -1190,15 +1190,6 @@ __global__ void __launch_bounds__(256) weight_grad_finish_kernel(WeightGradArgs 
   }
 }
 
-template <class F>
-int by_dtype(int dtype, F f) {
-  switch (dtype) {
-    case OPTIMI_F32: return f(std::integral_constant<int, OPTIMI_F32>{});
-    case OPTIMI_BF16: return f(std::integral_constant<int, OPTIMI_BF16>{});
-    default: return f(std::integral_constant<int, OPTIMI_F16>{});
-  }
-}
-
 constexpr int64_t kMostWidth = 1 << 24;  // of a weight gradient: offsets inside a tile stay in 31 bits
 constexpr int64_t kMostSum = 131071;  // (-128)^2 times this stays below 2^31
 // A launch holds fewer than 2^32 lanes.
@@ -1276,8 +1267,8 @@ inline int64_t padded(int64_t bytes) { return (bytes + 15) / 16 * 16; }
 // What a product of these sizes does: computed alike by the call and by its workspace function.
 //
 // Odd widths: large tiles are copied asynchronously and take padded copies of both operands.  Small ones can be loaded through registers,
-// at 0.45 us a step instead of 0.2; the copies cost a launch and 0.5 us per million bytes (measured: 42 x 216 x 3675 16.6 us through
-// registers, 13.3 us padded; 20 x 8000 x 8001 32 us, 38 us).
+// at 0.44 us a step instead of 0.17 to 0.20 (517 x 1001 and 1000 x 1000, k from 1024 to 8192); the copies cost a launch and 0.5 us per million
+// bytes (42 x 216 x 3675: 16.6 us through registers, 13.3 us padded; 20 x 8000 x 8001: 32 us, 38 us).
 inline int64_t vec_blocks(int64_t n, bool share) { return share ? (n + 3) / 4 : (n + 15) / 16; }
 struct MatmulPlan {
   bool vec;         // read off the weight

@@ -3,10 +3,10 @@
 //
 // All of them stream: every input is read once, every output written once, and HBM bandwidth is the bound.  What
 // stands in the way is that a row's scale (and the norm's 1/rms) is known only after the whole row was seen.  A row
-// therefore stays in the registers of the team of lanes that works on it - one wavefront for short rows, a workgroup
-// of four for longer ones - between the reduction and the use of its result; only rows beyond 16384 elements are
-// read again (the second read is served by L2).  Sums, the norm's statistics and the quantized values are formed in
-// fp32 whatever the type of the tensors.
+// therefore stays in the registers of the team of lanes that works on it - one wavefront for rows of up to 1024 elements, a
+// workgroup of four for up to 8192, of eight for up to 16384 - between the reduction and the use of its result; only rows beyond
+// 16384 elements are read again (the second read is served by L2).  Sums, the norm's statistics and the quantized values are
+// formed in fp32 whatever the type of the tensors.
 //
 // Measured (bf16; bytes that have to move / kernel time): quantize 16384 x 11008 88 us, 6.2 TB/s; norm with residual
 // 8192 x 4096 41 us, 5.7 TB/s; its backward pass 42 us + 4.5 us for the join of the partial sums, 6.4 TB/s; quantizing and
@@ -86,7 +86,7 @@ __global__ void __launch_bounds__(kLanes<TEAM>) quantize_kernel(const typename E
   constexpr bool kTiny = TEAM == 64 && VPT == 1;
   __shared__ uint32_t slots[2][kLanes<TEAM> / 64];
   const Place<TEAM> at;
-  // a team of four waves has the workgroup to itself, so all of its waves make the same number of rounds
+  // a team of several waves has the workgroup to itself, so all of its waves make the same number of rounds
   int turn = 0;
   for (int64_t row = at.row; row < rows; row += at.step, turn ^= 1) {
     const typename E::type* in = x + row * cols;
@@ -541,15 +541,6 @@ __global__ void __launch_bounds__(32 * kJoin) column_finish_kernel(const float* 
 // ------------------------------------------------------------------------------------
 // Host side
 // ------------------------------------------------------------------------------------
-
-template <class F>
-int by_dtype(int dtype, F f) {
-  switch (dtype) {
-    case OPTIMI_F32: return f(std::integral_constant<int, OPTIMI_F32>{});
-    case OPTIMI_BF16: return f(std::integral_constant<int, OPTIMI_BF16>{});
-    default: return f(std::integral_constant<int, OPTIMI_F16>{});
-  }
-}
 
 // Calls f(team, vectors per lane) for rows of `cols` elements that stay in registers.
 template <class F>
