@@ -347,13 +347,14 @@ int64_t optimi_hip_launch_limit(int64_t workgroups);
  * values[r][c] * scales[r].  The library's own scales are powers of two - the smallest s with
  * absmax <= 127 s, 1 for rows of zeros, never below 2^-126 - so a value's meaning is exact in every
  * type; values stay within +-63 under scales whose 64th multiple the type cannot hold.  A row
- * that holds an infinity or a NaN gets the scale NaN and zeros.  The products take any scales.
+ * that holds an infinity or a NaN gets the scale NaN and zeros.  The products take any scales (below 2^-126 with the bits
+ * that float32 has left there).
  *
  * All matrices are contiguous, rows < 2^31, cols <= 2^28 (outs and cols <= 2^24 for the weight
  * gradient), and a product has fewer than 2^24 tiles of 64 x 64 outputs (OPTIMI_ERR_SIZE beyond); where operands are
  * aligned to 16 bytes larger tiles carry it further (OPTIMI_ERR_ALIGN where only aligned ones would fit).  Buffers need
- * only be aligned to their element size; outputs overlap neither inputs nor each other.  Workspaces are the caller's: as many bytes of device memory
- * as the _workspace function of the same name and sizes says (it returns a negative status for
+ * only be aligned to their element size; outputs overlap neither inputs nor each other.  Workspaces are the caller's: as
+ * many bytes of device memory as the _workspace function of the same name and sizes says (it returns a negative status for
  * sizes that the call would refuse), aligned to 16 bytes, not shared by calls that may
  * run at the same time, free again when the call's work on `stream` is done; NULL where that is 0.
  * Nothing is allocated, cached or waited for, and every call may be captured into a HIP graph.
@@ -377,9 +378,11 @@ int optimi_hip_int8_matmul(const int8_t* a, const float* a_scales, const int8_t*
 /* The gradient of a linear layer's weight from the int8 checkpoint of its input:
  * weight_grad[n][k] = sum_r grad[r][n] * scales[r] * values[r][k], and bias_grad[n] = sum_r grad[r][n] where bias_grad
  * is not NULL.  grad [rows, outs], values [rows, cols], weight_grad [outs, cols]; all but values and scales are of
- * `dtype`.  Products of bf16 and fp16 gradients are formed with values[r][k] * scales[r] rounded to that type (exact
- * for this library's scales), those of fp32 gradients without rounding, where grad * scale lies between
- * 2^-110 and the largest float; sums are fp32.  rows = 0 writes zeros; cols = 0 leaves the
+ * `dtype`.  Products of bf16 and fp16 gradients are formed with values[r][k] * scales[r] rounded to that type: exact in
+ * bf16 for scales that are powers of two, and in fp16 where these numbers are also multiples of 2^-24 and within 65504, as
+ * those quantized from fp16 are (those of a norm or of another type need not be: smaller ones lose bits, larger ones become
+ * infinite).  Products of fp32 gradients are exact where grad * scale lies between 2^-110 and the largest float, but for
+ * one rounding of grad * scale if the scale is no power of two; sums are fp32.  rows = 0 writes zeros; cols = 0 leaves the
  * bias gradient, for which values, scales and weight_grad may be NULL. */
 int64_t optimi_hip_int8_weight_grad_workspace(int64_t rows, int64_t outs, int64_t cols, int dtype, int with_bias);
 int optimi_hip_int8_weight_grad(const void* grad, const int8_t* values, const float* scales, int64_t rows, int64_t outs,
@@ -388,7 +391,8 @@ int optimi_hip_int8_weight_grad(const void* grad, const int8_t* values, const fl
 
 /* h = x + residual (rounded to `dtype`; x itself, and h not written, where residual is NULL),
  * rstd[r] = 1 / sqrt(mean(h[r]^2) + eps), also where squares leave fp32's range, and the int8 form of
- * y[r][c] = h[r][c] * rstd[r] * weight[c], which is formed in fp32 and not rounded before.  weight is of `weight_dtype`: `dtype` or OPTIMI_F32.  cols >= 1. */
+ * y[r][c] = h[r][c] * rstd[r] * weight[c], which is formed in fp32 and not rounded before.  weight is of `weight_dtype`:
+ * `dtype` or OPTIMI_F32.  cols >= 1. */
 int optimi_hip_add_rms_norm_int8(const void* x, const void* residual, const void* weight, int64_t rows, int64_t cols,
                                  int dtype, int weight_dtype, double eps, void* h, int8_t* values, float* scales, float* rstd,
                                  optimi_stream_t stream);
